@@ -14,6 +14,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -23,10 +24,18 @@ CUDA_HOME = os.path.dirname(os.path.dirname(NVCC))
 LIB = os.path.join(PKG, "libffa_b200.so")
 EXT = os.path.join(PKG, "ff_attention" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
-CUDA_SOURCES = ["ffa_decode_kernels.cu", "ffa_c_api.cu", "ffa_no_alloc.cu", "ffa_peer_gather.cu"]
-KERNEL_HEADERS = ["ffa_internal.h", "ffa_device_common.cuh", "ffa_stream_kernel.cuh", "ffa_prune_kernels.cuh",
-                  "ffa_prune_stream_kernel.cuh"]
-CUDA_DEPS = CUDA_SOURCES + KERNEL_HEADERS + [os.path.join(ROOT, "include", "ffa_c_api.h")]
+API_HEADER = os.path.join(ROOT, "include", "ffa_c_api.h")
+COMMON_HEADERS = ["ffa_internal.h", "ffa_device_common.cuh", "ffa_launch.cuh"]
+# every source with the headers it includes: what makes its object stale
+CUDA_SOURCES = {
+    "ffa_decode_kernels.cu": [*COMMON_HEADERS, "ffa_stream_kernel.cuh", "ffa_prune_kernels.cuh", "ffa_prune_stream_kernel.cuh"],
+    "ffa_tree_kernels.cu": [*COMMON_HEADERS, "ffa_tree_kernel.cuh"],
+    "ffa_tree_api.cu": ["ffa_internal.h", "ffa_plan.h", API_HEADER],
+    "ffa_c_api.cu": ["ffa_internal.h", "ffa_plan.h", API_HEADER],
+    "ffa_no_alloc.cu": ["ffa_internal.h", API_HEADER],
+    "ffa_peer_gather.cu": COMMON_HEADERS,
+}
+CUDA_DEPS = sorted({*CUDA_SOURCES, *(h for deps in CUDA_SOURCES.values() for h in deps)})
 NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr"]
 
@@ -45,15 +54,16 @@ def _run(cmd) -> None:
 
 def build_library(force: bool = False, verbose_ptxas: bool = False) -> str:
     if force or _stale(LIB, CUDA_DEPS):
-        objs = []
-        for src in CUDA_SOURCES:
+        os.makedirs(os.path.join(PKG, "build"), exist_ok=True)
+        objs, cmds = [], []
+        for src, headers in CUDA_SOURCES.items():
             obj = os.path.join(PKG, "build", src.replace(".cu", ".o"))
-            os.makedirs(os.path.dirname(obj), exist_ok=True)
-            if force or _stale(obj, CUDA_DEPS if src != "ffa_decode_kernels.cu" else
-                               ["ffa_decode_kernels.cu"] + KERNEL_HEADERS):
-                _run([NVCC, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose_ptxas else []), "-c",
-                      os.path.join(CSRC, src), "-o", obj])
+            if force or _stale(obj, [src, *headers]):
+                cmds.append([NVCC, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose_ptxas else []), "-c",
+                             os.path.join(CSRC, src), "-o", obj])
             objs.append(obj)
+        with ThreadPoolExecutor(max(1, os.cpu_count() or 1)) as pool:
+            list(pool.map(_run, cmds))
         _run([NVCC, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", LIB, *objs])
     return LIB
 

@@ -15,6 +15,7 @@
 
 #include "../../include/ffa_c_api.h"
 #include "ffa_internal.h"
+#include "ffa_plan.h"
 
 namespace {
 
@@ -58,37 +59,8 @@ constexpr long long kAlignedBelowUnitsPerSlot = 200;
 // default only where it can win by 9 % or more.
 constexpr double kStreamPruneAboveBytes = 1e9;
 
-}  // namespace
-
-struct ffa_plan {
-    int dtype, B, H, Dh, Lmax, use_default, device, mode;
-    int prune_path;  // 0 = choose, 1 = fused cluster kernel only, 2 = streaming kernel only
-    int cluster_merge;  // 1 = merge split pairs inside a thread-block cluster when the cut allows it
-    // answers of the occupancy query for cluster launches, keyed by (threads, shared memory, cluster size)
-    struct { int threads, smem, cluster, clusters; } occ[8];
-    int occ_n;
-    bool offline;    // planning only: created from given device properties, never launches
-    int sms, smem_per_cta, smem_per_sm;
-    bool forced;
-    ffa_launch_t force;
-    // workspace carving
-    void* ws;
-    size_t ws_bytes;
-    int* status;
-    int* tickets;
-    float* partials;
-    float* scores;
-    int max_grid;
-    // output gather over peer memory
-    int peer_world, peer_rank;
-    void* peer_buf[FFA_MAX_PEERS];
-    void* push_gathered;   // non-null: exact steps push their output rows to the peers (ffa_peer_push_target)
-};
-
-namespace {
-
 struct Carve {
-    size_t status, tickets, partials, scores, total;
+    size_t status, tickets, tree_tickets, partials, scores, total;
 };
 Carve carve(const ffa_plan* p, bool with_scores)
 {
@@ -97,6 +69,7 @@ Carve carve(const ffa_plan* p, bool with_scores)
     size_t off = 0;
     c.status = off, off += 256;
     c.tickets = off, off += align_up(BH * sizeof(int), 256);
+    c.tree_tickets = off, off += align_up(BH * kTreeTicketsPerPair * sizeof(int), 256);
     c.partials = off, off += align_up(((size_t)p->max_grid + BH) * (p->Dh + 2) * sizeof(float), 256);
     c.scores = off;
     if (with_scores) off += align_up(BH * (size_t)score_stride(p->Lmax) * sizeof(float), 256);
@@ -373,6 +346,17 @@ int fit_clusters(ffa_plan* plan, int cap, bool paged, ffa_launch_t* L, int* clus
 
 }  // namespace
 
+int ffa_fail(int code, const char* fmt, ...)
+{
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+int ffa_cuda_fail(int e, const char* what) { return cuda_fail(e, what); }
+void ffa_count_launches(int n) { g_launches.fetch_add((unsigned long long)n); }
+
 extern "C" {
 
 const char* ffa_last_error(void) { return g_err; }
@@ -438,6 +422,7 @@ int ffa_plan_create(int dtype, int batch, int heads, int head_dim, int max_len, 
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&smem_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, device);
     int r = 0;
     if (e == cudaSuccess) r = ffa_k_prepare(dtype, head_dim, smem_cta);
+    if (e == cudaSuccess && r == 0) r = ffa_k_tree_prepare(dtype, head_dim);
     cudaSetDevice(prev);
     if (e != cudaSuccess) return cuda_fail(e, "device attribute query");
     if (r != 0) return cuda_fail(r, "kernel preparation (is this an sm_100a device?)");
@@ -566,6 +551,7 @@ int ffa_workspace_bind(ffa_plan_t* plan, void* workspace, size_t bytes, void* st
     plan->ws = workspace, plan->ws_bytes = bytes;
     plan->status = reinterpret_cast<int*>(base + small.status);
     plan->tickets = reinterpret_cast<int*>(base + small.tickets);
+    plan->tree_tickets = reinterpret_cast<int*>(base + small.tree_tickets);
     plan->partials = reinterpret_cast<float*>(base + small.partials);
     plan->scores = bytes >= big.total ? reinterpret_cast<float*>(base + big.scores) : nullptr;
     return FFA_OK;

@@ -36,6 +36,7 @@
 
 #include "ffa_internal.h"
 #include "ffa_device_common.cuh"
+#include "ffa_launch.cuh"
 #include "ffa_prune_kernels.cuh"
 #include "ffa_prune_stream_kernel.cuh"
 #include "ffa_stream_kernel.cuh"
@@ -87,29 +88,6 @@ __global__ void __launch_bounds__(32) ffa_wait_selftest_kernel(int* status, unsi
         if (!ok || dead) atomicOr(status, kStatusWaitTimeout);
         if (waited_ns != nullptr) *waited_ns = global_timer_ns() - t0;
     }
-}
-
-// ------------------------------------------------------------------------------------------
-// Host-side dispatch
-// ------------------------------------------------------------------------------------------
-template <typename F>
-int dispatch(int dtype, int head_dim, F&& f)
-{
-#define FFA_DH_SWITCH(T)                                        \
-    switch (head_dim) {                                         \
-        case 64: return f(T{}, std::integral_constant<int, 64>{});   \
-        case 80: return f(T{}, std::integral_constant<int, 80>{});   \
-        case 128: return f(T{}, std::integral_constant<int, 128>{}); \
-        case 256: return f(T{}, std::integral_constant<int, 256>{}); \
-        default: return (int)cudaErrorInvalidValue;             \
-    }
-    switch (dtype) {
-        case 0: FFA_DH_SWITCH(float)
-        case 1: FFA_DH_SWITCH(__half)
-        case 2: FFA_DH_SWITCH(__nv_bfloat16)
-        default: return (int)cudaErrorInvalidValue;
-    }
-#undef FFA_DH_SWITCH
 }
 
 int elem_size(int dtype) { return dtype == 0 ? 4 : 2; }
@@ -195,34 +173,6 @@ int ffa_k_wait_selftest(int* status, unsigned long long limit_ns, unsigned long 
 // 9.2 us with it); above, an early start of the next grid's CTAs costs more than it hides (2 K tokens 161.8 vs 156.0 us,
 // 8 K 605.8 vs 593.6 us)
 constexpr double kPdlBelowBytes = 512e6;
-
-// Launch -- when `overlap`, with the programmatic-serialisation attribute: the kernel may start while the previous
-// kernel of the stream drains and waits at pdl_wait() before touching global memory -- and, when cluster > 1, as
-// thread-block clusters of that many CTAs.
-template <typename K>
-cudaError_t launch_pdl(K kernel, int grid, int threads, int smem, int cluster, bool overlap, cudaStream_t stream, const FfaStepParams& P)
-{
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)grid, 1, 1);
-    cfg.blockDim = dim3((unsigned)threads, 1, 1);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (overlap) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
-    if (cluster > 1) {
-        attr[n].id = cudaLaunchAttributeClusterDimension;
-        attr[n].val.clusterDim.x = (unsigned)cluster, attr[n].val.clusterDim.y = 1, attr[n].val.clusterDim.z = 1;
-        ++n;
-    }
-    cfg.attrs = attr, cfg.numAttrs = (unsigned)n;
-    return cudaLaunchKernelEx(&cfg, kernel, P);
-}
 
 int ffa_k_decode_onepass(int dtype, int head_dim, const FfaStepParams& P, int threads, int smem, cudaStream_t stream)
 {

@@ -20,6 +20,7 @@ constexpr uint32_t kDrainPolls = 1u << 20;
 constexpr int kMaxClusterCtas = 8;   // portable thread-block cluster size
 constexpr int kStatusWaitTimeout = 1;
 constexpr int kStatusBadLength = 2;
+constexpr int kStatusBadIndex = 4;
 
 // ------------------------------------------------------------------------------------------
 // PTX wrappers: mbarrier + 1-D bulk copy global -> this CTA's shared memory
@@ -102,6 +103,17 @@ __device__ __forceinline__ void bulk_copy_g2s(uint32_t dst, const void* src, uin
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// same, but `bytes` (0 or 16) are read and the rest of the slot is filled with zeros
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, uint32_t bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all()
 {
@@ -288,7 +300,8 @@ struct SampleRange {
     int first, row;
     bool ok;
 };
-__device__ __forceinline__ SampleRange sample_range(const FfaStepParams& P, int b)
+template <typename Params>   // FfaStepParams or FfaTreeParams
+__device__ __forceinline__ SampleRange sample_range(const Params& P, int b)
 {
     SampleRange r;
     r.first = 0, r.row = P.t;
@@ -308,7 +321,8 @@ __device__ __forceinline__ SampleRange sample_range(const FfaStepParams& P, int 
 // page_table[b][row / page_rows] names the page; rows of one (pair, page) are contiguous, and
 // the streaming kernel's tiles never straddle pages because tile_rows divides page_rows (the
 // fused pruning kernel splits a tile's copy at page boundaries instead).
-__device__ __forceinline__ size_t cache_row_offset(const FfaStepParams& P, int bh, int row, int rowb)
+template <typename Params>   // FfaStepParams, FfaTreeParams or FfaAcceptParams
+__device__ __forceinline__ size_t cache_row_offset(const Params& P, int bh, int row, int rowb)
 {
     if (P.page_table == nullptr) return ((size_t)bh * P.Lmax + row) * rowb;
     const int b = bh / P.H, h = bh - b * P.H;

@@ -84,3 +84,47 @@ int ffa_k_fused_smem_bytes(int dtype, int head_dim, int tile_rows, int stages, i
 int ffa_k_wait_selftest(int* status, unsigned long long limit_ns, unsigned long long* waited_ns, cudaStream_t stream);
 // all-gather of the step outputs: a few CTAs per rank
 int ffa_k_peer_gather(FfaPeerGatherParams G, cudaStream_t stream);
+
+// Arrival counters per pair: one per tile of query rows of a tree attention (at most 1024 rows, tiles of 32 or more; 8 rows only
+// where a pair has no more than 8).
+constexpr int kTreeTicketsPerPair = 32;
+constexpr int kTreeMaxRows = 1024;   // groups * tokens
+
+// One attention step for a tree of drafted tokens (ffa_tree_attention).  Rows r = g * tokens + t of a pair are query head
+// h * groups + g at drafted token t.
+struct FfaTreeParams {
+    const void* q;     // [B, H*groups, tokens, Dh]
+    const void* k;     // [B, H, tokens, Dh]
+    const void* v;     // [B, H, tokens, Dh]
+    void* k_cache;     // [B*H, Lmax, Dh] or the page pool
+    void* v_cache;
+    void* out;         // [B, H*groups, tokens, Dh]
+    const unsigned char* tree;   // [tokens, tokens] or [B, tokens, tokens]: nonzero = row t sees drafted token j
+    int tree_per_sample;
+    const int* seq_lengths;      // as in FfaStepParams
+    int right_or_no_padding;
+    int B, H, Lmax, t, groups, tokens;
+    float scale;
+    int splits, row_tiles;       // CTAs per (pair, tile of query rows); tiles of query rows per pair
+    float* partials;             // [B*H][row_tiles][splits][tile rows][Dh + 2]; null when splits == 1
+    int* tickets;                // [B*H][kTreeTicketsPerPair], zero between launches
+    int* status;
+    const int* page_table;       // as in FfaStepParams
+    int max_pages, page_rows;
+};
+// Moving the accepted path of a tree to the front of its rows (ffa_tree_accept).
+struct FfaAcceptParams {
+    void* k_cache;
+    void* v_cache;
+    const int* path;             // [B, path_len]: increasing tree indices, then -1
+    const int* seq_lengths;      // [B] or null
+    int path_len, B, H, Lmax, t, row_bytes;
+    int* status;
+    const int* page_table;
+    int max_pages, page_rows;
+};
+int ffa_k_tree_rows(int dtype, int rows);      // query rows per CTA
+int ffa_k_tree_smem(int dtype, int head_dim, int rows);
+int ffa_k_tree_prepare(int dtype, int head_dim);
+int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaStream_t stream);
+int ffa_k_tree_accept(const FfaAcceptParams& P, cudaStream_t stream);

@@ -1,0 +1,137 @@
+// C entries of the tree attention (include/ffa_c_api.h): argument checks, the cut over CTAs and the parameter fill.
+#include <cuda_runtime.h>
+
+#include <cstring>
+
+#include "../../include/ffa_c_api.h"
+#include "ffa_internal.h"
+#include "ffa_plan.h"
+
+namespace {
+
+// The cut of a tree attention: tiles of query rows per pair, and CTAs per (pair, tile of query rows).
+struct TreeShape {
+    int tile_rows, row_tiles, splits;
+};
+
+TreeShape tree_shape(const ffa_plan* p, int groups, int tokens, int t)
+{
+    TreeShape s;
+    const int rows = groups * tokens;
+    s.tile_rows = ffa_k_tree_rows(p->dtype, rows);
+    s.row_tiles = (rows + s.tile_rows - 1) / s.tile_rows;
+    // two CTAs per SM; a split has at least four key tiles
+    const long long items = (long long)p->B * p->H * s.row_tiles;
+    const long long tiles = (t + 31) / 32 + (tokens + 31) / 32;
+    long long splits = 2LL * p->sms / items;
+    if (splits > tiles / 4) splits = tiles / 4;
+    s.splits = (int)(splits < 1 ? 1 : splits);
+    return s;
+}
+
+size_t tree_partials_bytes(const ffa_plan* p, const TreeShape& s)
+{
+    if (s.splits <= 1) return 0;
+    return (size_t)p->B * p->H * s.row_tiles * s.splits * s.tile_rows * (p->Dh + 2) * sizeof(float);
+}
+
+int check_sizes(const ffa_plan* plan, int groups, int tokens, int t)
+{
+    if (plan == nullptr) return ffa_fail(FFA_ERR_ARG, "null plan");
+    if (groups <= 0 || tokens <= 0) return ffa_fail(FFA_ERR_RANGE, "groups (%d) and tokens (%d) must be positive", groups, tokens);
+    if (tokens > kTreeMaxRows || groups > kTreeMaxRows || groups * tokens > kTreeMaxRows)
+        return ffa_fail(FFA_ERR_RANGE, "groups * tokens (%d * %d) exceeds %d query rows per cache head", groups, tokens, kTreeMaxRows);
+    if (t < 0 || t >= plan->Lmax) return ffa_fail(FFA_ERR_RANGE, "t = %d outside [0, %d)", t, plan->Lmax);
+    if ((long long)plan->B * plan->H * groups * tokens >= (1LL << 31)) return ffa_fail(FFA_ERR_RANGE, "sizes exceed int range");
+    return FFA_OK;
+}
+
+int check_pages(const ffa_plan* plan, const int* page_table, int max_pages, int page_rows)
+{
+    if (page_table == nullptr) return FFA_OK;
+    if (page_rows <= 0 || page_rows % 128 != 0)
+        return ffa_fail(FFA_ERR_RANGE, "page_rows (%d) must be a positive multiple of 128", page_rows);
+    if (max_pages <= 0 || (long long)max_pages * page_rows != plan->Lmax)
+        return ffa_fail(FFA_ERR_RANGE, "max_pages * page_rows (%d * %d) must equal the plan's max_len (%d)", max_pages, page_rows, plan->Lmax);
+    return FFA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ffa_tree_scratch_bytes(const ffa_plan_t* plan, int groups, int tokens, int t, size_t* bytes)
+{
+    const int r = check_sizes(plan, groups, tokens, t);
+    if (r != FFA_OK) return r;
+    if (bytes == nullptr) return ffa_fail(FFA_ERR_ARG, "null output pointer");
+    *bytes = tree_partials_bytes(plan, tree_shape(plan, groups, tokens, t));
+    return FFA_OK;
+}
+
+int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                       const unsigned char* tree, int tree_per_sample, int groups, int tokens, void* out, float softmax_scale, int t,
+                       const int* seq_lengths, int right_or_no_padding, const int* page_table, int max_pages, int page_rows,
+                       void* scratch, size_t scratch_bytes, void* stream)
+{
+    int r = check_sizes(plan, groups, tokens, t);
+    if (r != FFA_OK) return r;
+    if (!q || !k || !v || !k_cache || !v_cache || !tree || !out) return ffa_fail(FFA_ERR_ARG, "null tensor pointer");
+    if (!ffa_aligned16(q) || !ffa_aligned16(k) || !ffa_aligned16(v) || !ffa_aligned16(k_cache) || !ffa_aligned16(v_cache) || !ffa_aligned16(out))
+        return ffa_fail(FFA_ERR_ARG, "tensor pointers must be 16-byte aligned");
+    if (seq_lengths == nullptr && !right_or_no_padding)
+        return ffa_fail(FFA_ERR_ARG, "left padding (right_or_no_padding = 0) needs seq_lengths");
+    if ((seq_lengths == nullptr || !right_or_no_padding) && tokens > plan->Lmax - t)
+        return ffa_fail(FFA_ERR_RANGE, "t + tokens (%d + %d) exceeds the cache length %d", t, tokens, plan->Lmax);
+    r = check_pages(plan, page_table, max_pages, page_rows);
+    if (r != FFA_OK) return r;
+    if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
+    if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
+    const TreeShape s = tree_shape(plan, groups, tokens, t);
+    const size_t need = tree_partials_bytes(plan, s);
+    if (need > 0 && (scratch == nullptr || scratch_bytes < need))
+        return ffa_fail(FFA_ERR_WORKSPACE, "scratch of %zu bytes, need %zu (ffa_tree_scratch_bytes)", scratch ? scratch_bytes : (size_t)0, need);
+    if (need > 0 && !ffa_aligned16(scratch)) return ffa_fail(FFA_ERR_ARG, "scratch must be 16-byte aligned");
+    if ((long long)plan->B * plan->H * s.row_tiles * s.splits >= (1LL << 31)) return ffa_fail(FFA_ERR_RANGE, "sizes exceed int range");
+    FfaTreeParams P;
+    std::memset(&P, 0, sizeof(P));
+    P.q = q, P.k = k, P.v = v, P.k_cache = k_cache, P.v_cache = v_cache, P.out = out;
+    P.tree = tree, P.tree_per_sample = tree_per_sample != 0;
+    P.seq_lengths = seq_lengths, P.right_or_no_padding = right_or_no_padding != 0;
+    P.B = plan->B, P.H = plan->H, P.Lmax = plan->Lmax, P.t = t, P.groups = groups, P.tokens = tokens;
+    P.scale = softmax_scale;
+    P.splits = s.splits, P.row_tiles = s.row_tiles;
+    P.partials = static_cast<float*>(scratch), P.tickets = plan->tree_tickets, P.status = plan->status;
+    P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows;
+    r = ffa_k_tree_attention(plan->dtype, plan->Dh, P, static_cast<cudaStream_t>(stream));
+    if (r != 0) return ffa_cuda_fail(r, "tree attention launch");
+    ffa_count_launches(1);
+    return FFA_OK;
+}
+
+int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* path, int path_len, int t, const int* seq_lengths,
+                    const int* page_table, int max_pages, int page_rows, void* stream)
+{
+    if (plan == nullptr) return ffa_fail(FFA_ERR_ARG, "null plan");
+    if (path_len < 0 || path_len > kTreeMaxRows) return ffa_fail(FFA_ERR_RANGE, "path length %d outside [0, %d]", path_len, kTreeMaxRows);
+    if (t < 0 || t >= plan->Lmax) return ffa_fail(FFA_ERR_RANGE, "t = %d outside [0, %d)", t, plan->Lmax);
+    if (!k_cache || !v_cache || (path_len > 0 && !path)) return ffa_fail(FFA_ERR_ARG, "null tensor pointer");
+    if (!ffa_aligned16(k_cache) || !ffa_aligned16(v_cache)) return ffa_fail(FFA_ERR_ARG, "tensor pointers must be 16-byte aligned");
+    int r = check_pages(plan, page_table, max_pages, page_rows);
+    if (r != FFA_OK) return r;
+    if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
+    if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
+    if (path_len == 0) return FFA_OK;
+    FfaAcceptParams P;
+    std::memset(&P, 0, sizeof(P));
+    P.k_cache = k_cache, P.v_cache = v_cache, P.path = path, P.seq_lengths = seq_lengths, P.path_len = path_len;
+    P.B = plan->B, P.H = plan->H, P.Lmax = plan->Lmax, P.t = t, P.row_bytes = plan->Dh * ffa_elem_size(plan->dtype);
+    P.status = plan->status;
+    P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows;
+    r = ffa_k_tree_accept(P, static_cast<cudaStream_t>(stream));
+    if (r != 0) return ffa_cuda_fail(r, "tree accept launch");
+    ffa_count_launches(1);
+    return FFA_OK;
+}
+
+}  // extern "C"

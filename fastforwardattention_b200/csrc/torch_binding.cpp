@@ -36,6 +36,89 @@ int dtype_code(const torch::Tensor& x)
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == FFA_OK, "FastForwardAttn: ", what, ": ", ffa_last_error()); }
 
+// What a tree attention or acceptance works on: an engine's plan and its caches, contiguous or paged.
+struct TreeTarget {
+    const char* who;
+    ffa_plan_t* plan;
+    c10::Device device;
+    int dtype;
+    int64_t B, H, Dh;
+    torch::Tensor k, v;              // caches or page pools
+    const torch::Tensor* table;      // [B, max_pages] or null
+    int64_t max_pages, page_rows;
+    const int* table_ptr() const { return table ? table->data_ptr<int>() : nullptr; }
+};
+
+torch::Tensor checked_rows(const TreeTarget& T, const torch::Tensor& rows, const char* name)
+{
+    TORCH_CHECK(rows.is_cuda() && rows.device() == T.device && rows.scalar_type() == torch::kInt && rows.numel() == T.B, T.who, ": ", name,
+                " must be an int32 CUDA tensor with one entry per batch element");
+    return rows.contiguous();
+}
+
+void check_table(const TreeTarget& T)
+{
+    if (T.table == nullptr) return;
+    TORCH_CHECK(T.table->is_cuda() && T.table->device() == T.device && T.table->scalar_type() == torch::kInt && T.table->is_contiguous() &&
+                    T.table->dim() == 2 && T.table->size(0) == T.B && T.table->size(1) == T.max_pages,
+                T.who, ": page_table must be a contiguous int32 CUDA tensor [batch, max_pages]");
+}
+
+// rows: per-sample lengths (right padding), or with left_padding the count of masked keys of every sample
+torch::Tensor run_tree(const TreeTarget& T, const torch::Tensor& q_, const torch::Tensor& k_, const torch::Tensor& v_, const torch::Tensor& tree_,
+                       double softmax_scale, int64_t t, const torch::Tensor* rows_, bool left_padding, c10::optional<torch::Tensor> out_opt)
+{
+    TORCH_CHECK(tree_.is_cuda() && tree_.device() == T.device && (tree_.scalar_type() == torch::kBool || tree_.scalar_type() == torch::kByte) &&
+                    (tree_.dim() == 2 || (tree_.dim() == 3 && tree_.size(0) == T.B)) && tree_.size(-1) == tree_.size(-2) && tree_.size(-1) > 0,
+                T.who, ": tree must be a bool CUDA tensor [tokens, tokens] or [batch, tokens, tokens]");
+    const int64_t n = tree_.size(-1);
+    TORCH_CHECK(q_.dim() == 4 && q_.size(0) == T.B && q_.size(1) > 0 && q_.size(1) % T.H == 0 && q_.size(2) == n && q_.size(3) == T.Dh, T.who,
+                ": q must be [batch, a multiple of ", T.H, " heads, ", n, " tokens, ", T.Dh, "]");
+    const int64_t groups = q_.size(1) / T.H;
+    TORCH_CHECK(n <= 1024 && groups * n <= 1024, T.who, ": groups * tokens (", groups, " * ", n, ") exceeds 1024 query rows per cache head");
+    auto prep = [&](const torch::Tensor& x, const char* name, int64_t heads) {
+        TORCH_CHECK(x.is_cuda() && x.device() == T.device && dtype_code(x) == T.dtype, T.who, ": ", name,
+                    " must be a CUDA tensor of the cache's dtype on the cache's device");
+        TORCH_CHECK(x.dim() == 4 && x.size(0) == T.B && x.size(1) == heads && x.size(2) == n && x.size(3) == T.Dh, T.who, ": ", name,
+                    " must be [", T.B, ", ", heads, ", ", n, ", ", T.Dh, "]");
+        return x.contiguous();
+    };
+    torch::Tensor q = prep(q_, "q", T.H * groups), k = prep(k_, "k", T.H), v = prep(v_, "v", T.H), tree = tree_.contiguous(), rows;
+    if (rows_ != nullptr) rows = checked_rows(T, *rows_, "seq_lengths");
+    check_table(T);
+    c10::cuda::CUDAGuard guard(T.device);
+    torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty_like(q, torch::MemoryFormat::Contiguous);
+    TORCH_CHECK(out.is_cuda() && out.device() == T.device && dtype_code(out) == T.dtype && out.is_contiguous() && out.sizes() == q.sizes(), T.who,
+                ": out must be a contiguous tensor of q's shape and dtype on the cache's device");
+    size_t bytes = 0;
+    check(ffa_tree_scratch_bytes(T.plan, (int)groups, (int)n, (int)t, &bytes), "tree attention");
+    torch::Tensor scratch;   // this call's own, from the stream's allocator: nothing is shared with other calls or captured graphs
+    if (bytes > 0) scratch = torch::empty({(int64_t)bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(T.device));
+    check(ffa_tree_attention(T.plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), T.k.data_ptr(), T.v.data_ptr(),
+                             static_cast<const unsigned char*>(tree.data_ptr()), tree.dim() == 3, (int)groups, (int)n, out.data_ptr(),
+                             (float)softmax_scale, (int)t, rows_ ? rows.data_ptr<int>() : nullptr, !left_padding, T.table_ptr(),
+                             (int)T.max_pages, (int)T.page_rows, bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                             at::cuda::getCurrentCUDAStream().stream()),
+          "tree attention");
+    return out;
+}
+
+void run_accept(const TreeTarget& T, const torch::Tensor& path_, int64_t t, const torch::Tensor* rows_)
+{
+    TORCH_CHECK(path_.is_cuda() && path_.device() == T.device && path_.scalar_type() == torch::kInt && path_.dim() == 2 && path_.size(0) == T.B &&
+                    path_.size(1) <= 1024,
+                T.who, ": path must be an int32 CUDA tensor [batch, at most 1024 tree indices]");
+    torch::Tensor path = path_.contiguous(), rows;
+    if (rows_ != nullptr) rows = checked_rows(T, *rows_, "seq_lengths");
+    check_table(T);
+    c10::cuda::CUDAGuard guard(T.device);
+    torch::Tensor k = T.k, v = T.v;
+    check(ffa_tree_accept(T.plan, k.data_ptr(), v.data_ptr(), path.numel() > 0 ? path.data_ptr<int>() : nullptr, (int)path.size(1), (int)t,
+                          rows_ ? rows.data_ptr<int>() : nullptr, T.table_ptr(), (int)T.max_pages, (int)T.page_rows,
+                          at::cuda::getCurrentCUDAStream().stream()),
+          "tree accept");
+}
+
 struct FastForwardAttn {
     FastForwardAttn(torch::Tensor K, torch::Tensor V, int64_t max_timesteps, bool use_default_kernel_launch)
     {
@@ -276,6 +359,28 @@ struct FastForwardAttn {
                    gather_into);
     }
 
+    // ---- trees of drafted tokens (ffa_tree_attention, ffa_tree_accept) ----
+    TreeTarget target() const { return TreeTarget{"FastForwardAttn", plan, device, dtype, B, H, Dh, k_cache, v_cache, nullptr, 0, 0}; }
+    torch::Tensor tree_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor tree, double softmax_scale,
+                                 int64_t curr_timestep, c10::optional<torch::Tensor> seq_lengths, c10::optional<torch::Tensor> out)
+    {
+        TORCH_CHECK(curr_timestep >= 0 && curr_timestep < Lmax, "FastForwardAttn: curr_timestep ", curr_timestep, " outside [0, ", Lmax, ")");
+        return run_tree(target(), q, k, v, tree, softmax_scale, curr_timestep, seq_lengths.has_value() ? &*seq_lengths : nullptr,
+                        seq_lengths.has_value(), out);
+    }
+    torch::Tensor tree_attention_per_sample(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor tree, double softmax_scale,
+                                            torch::Tensor seq_lengths, c10::optional<torch::Tensor> out, int64_t max_row)
+    {
+        TORCH_CHECK(max_row >= -1 && max_row < Lmax, "FastForwardAttn: max_row ", max_row, " outside [-1, ", Lmax, ")");
+        return run_tree(target(), q, k, v, tree, softmax_scale, max_row < 0 ? Lmax - 1 : max_row, &seq_lengths, false, out);
+    }
+    void tree_accept(torch::Tensor path, int64_t curr_timestep)
+    {
+        TORCH_CHECK(curr_timestep >= 0 && curr_timestep < Lmax, "FastForwardAttn: curr_timestep ", curr_timestep, " outside [0, ", Lmax, ")");
+        run_accept(target(), path, curr_timestep, nullptr);
+    }
+    void tree_accept_per_sample(torch::Tensor path, torch::Tensor seq_lengths) { run_accept(target(), path, 0, &seq_lengths); }
+
     std::pair<torch::Tensor, torch::Tensor> get_cache() { return std::make_pair(k_cache, v_cache); }
 
     void set_mode(const std::string& m)
@@ -515,6 +620,18 @@ struct PagedEngine {
                     max_pages * page_rows, ")");
         return run(q, k, v, table, scale, max_row < 0 ? max_pages * page_rows - 1 : max_row, &rows, prob_thresh, out);
     }
+    TreeTarget target(const torch::Tensor& table) const
+    {
+        return TreeTarget{"PagedEngine", plan, device, dtype, B, H, Dh, kp, vp, &table, max_pages, page_rows};
+    }
+    torch::Tensor tree_attention_per_sample(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor tree, torch::Tensor table,
+                                            double scale, torch::Tensor rows, c10::optional<torch::Tensor> out, int64_t max_row)
+    {
+        const int64_t most = max_pages * page_rows;
+        TORCH_CHECK(max_row >= -1 && max_row < most, "PagedEngine: max_row ", max_row, " outside [-1, ", most, ")");
+        return run_tree(target(table), q, k, v, tree, scale, max_row < 0 ? most - 1 : max_row, &rows, false, out);
+    }
+    void tree_accept_per_sample(torch::Tensor path, torch::Tensor table, torch::Tensor rows) { run_accept(target(table), path, 0, &rows); }
     void set_mode(const std::string& m)
     {
         TORCH_CHECK(m == "exact" || m == "round_like_torch", "PagedEngine: mode must be 'exact' or 'round_like_torch'");
@@ -574,6 +691,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
              "decode step with per-sample cache lengths (right padding): sample b appends at row seq_lengths[b]", py::arg("q"),
              py::arg("k"), py::arg("v"), py::arg("softmax_scale"), py::arg("seq_lengths"), py::arg("prob_thresh") = 0.0,
              py::arg("out") = py::none(), py::arg("max_row") = -1, py::arg("gather_into") = py::none())
+        .def("tree_attention", &FastForwardAttn::tree_attention,
+             "attention of a tree of drafted tokens: q [B, G*H, T, Dh], k, v [B, H, T, Dh], tree [T, T] or [B, T, T] (row sees token); "
+             "appends k, v at rows curr_timestep..; seq_lengths: left padding, keys below seq_lengths[b] are masked",
+             py::arg("q"), py::arg("k"), py::arg("v"), py::arg("tree"), py::arg("softmax_scale"), py::arg("curr_timestep"),
+             py::arg("seq_lengths") = py::none(), py::arg("out") = py::none())
+        .def("tree_attention_per_sample", &FastForwardAttn::tree_attention_per_sample,
+             "tree attention with per-sample cache lengths: sample b appends at rows seq_lengths[b]..", py::arg("q"), py::arg("k"),
+             py::arg("v"), py::arg("tree"), py::arg("softmax_scale"), py::arg("seq_lengths"), py::arg("out") = py::none(),
+             py::arg("max_row") = -1)
+        .def("tree_accept", &FastForwardAttn::tree_accept,
+             "keep a verified path [B, A] (increasing tree indices, then -1): rows curr_timestep + path[b, i] -> curr_timestep + i",
+             py::arg("path"), py::arg("curr_timestep"))
+        .def("tree_accept_per_sample", &FastForwardAttn::tree_accept_per_sample, py::arg("path"), py::arg("seq_lengths"))
         .def("set_push_target", &FastForwardAttn::set_push_target, py::arg("gathered") = py::none(),
              "while set, exact steps push their output rows to the peers from the attention kernel (follow with peer_gather(phases=2))")
         .def("set_mode", &FastForwardAttn::set_mode, "'exact' (default) or 'round_like_torch'")
@@ -604,6 +734,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         .def("attention_per_sample", &PagedEngine::attention_per_sample, "decode step, sequence b at row rows[b]", py::arg("q"),
              py::arg("k"), py::arg("v"), py::arg("page_table"), py::arg("softmax_scale"), py::arg("rows"),
              py::arg("prob_thresh") = 0.0, py::arg("out") = py::none(), py::arg("max_row") = -1)
+        .def("tree_attention_per_sample", &PagedEngine::tree_attention_per_sample, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("tree"),
+             py::arg("page_table"), py::arg("softmax_scale"), py::arg("rows"), py::arg("out") = py::none(), py::arg("max_row") = -1)
+        .def("tree_accept_per_sample", &PagedEngine::tree_accept_per_sample, py::arg("path"), py::arg("page_table"), py::arg("rows"))
         .def("set_mode", &PagedEngine::set_mode, "'exact' (default) or 'round_like_torch'")
         .def("set_prune_path", &PagedEngine::set_prune_path, "0 choose, 1 cluster kernel, 2 streaming kernel")
         .def("record_kept_mask", &PagedEngine::record_kept_mask)

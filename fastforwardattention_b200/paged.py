@@ -95,6 +95,38 @@ class PagedFastForwardAttn:
         self.lengths = [n + 1 for n in self.lengths]
         return res
 
+    def tree_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, tree: torch.Tensor, softmax_scale: float,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of a tree of T drafted tokens (q [B, G*H, T, Dh], k, v [B, H, T, Dh], tree [T, T] or [B, T, T]): sequence b
+        writes k, v at rows lengths[b].. and its length stays as it was until tree_accept says which of them are kept."""
+        T = k.shape[2]
+        for b, n in enumerate(self.lengths):
+            if n + T > self.max_pages * self.pool.page_rows:
+                raise RuntimeError(f"sequence {b} has no room for {T} tokens ({self.max_pages * self.pool.page_rows} rows)")
+        for b, n in enumerate(self.lengths):
+            for row in range(n // self.pool.page_rows * self.pool.page_rows, n + T, self.pool.page_rows):
+                self._ensure_page(b, row)
+        return self.engine.tree_attention_per_sample(q, k, v, tree, self.table, softmax_scale, self.rows, out=out,
+                                                     max_row=max(self.lengths))
+
+    def tree_accept(self, path: Sequence[Sequence[int]]) -> None:
+        """Keeps path[b] (increasing indices into the tree of the last tree_attention) of every sequence: its rows move to the
+        end of the sequence, which grows by len(path[b]).  Pages taken for the rest of the tree stay with the sequence."""
+        A = max((len(p) for p in path), default=0)
+        if len(path) != self.B or any(list(p) != sorted(set(int(x) for x in p)) or (len(p) and p[0] < 0) for p in path):
+            raise ValueError("path must hold, for each sequence, increasing non-negative tree indices")
+        pr = self.pool.page_rows
+        for b, p in enumerate(path):
+            if len(p) and (self.lengths[b] + p[-1] >= self.max_pages * pr or self.table_host[b, (self.lengths[b] + p[-1]) // pr] < 0):
+                raise ValueError(f"path of sequence {b} names a token that was not drafted")
+        if A:
+            flat = torch.full((self.B, A), -1, dtype=torch.int32)
+            for b, p in enumerate(path):
+                flat[b, : len(p)] = torch.tensor(list(p), dtype=torch.int32)
+            self.engine.tree_accept_per_sample(flat.to(self.table.device), self.table, self.rows)
+            self.rows += torch.tensor([len(p) for p in path], dtype=torch.int32).to(self.rows.device)
+        self.lengths = [n + len(p) for n, p in zip(self.lengths, path)]
+
     @property
     def pages_in_use(self) -> int:
         return int((self.table_host >= 0).sum())

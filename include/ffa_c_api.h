@@ -49,7 +49,8 @@ enum {
 /* Bits of the device status word (ffa_device_status). */
 enum {
     FFA_STATUS_WAIT_TIMEOUT = 1, /* a bounded wait on a copy barrier ran out */
-    FFA_STATUS_BAD_LENGTH = 2    /* a per-sample length was outside [0, max_len) or above the stated bound */
+    FFA_STATUS_BAD_LENGTH = 2,   /* a per-sample length was outside [0, max_len) or above the stated bound */
+    FFA_STATUS_BAD_INDEX = 4     /* a row or beam index read from device memory was out of range; its sample was left as it was */
 };
 
 typedef struct ffa_plan ffa_plan_t;
@@ -172,6 +173,31 @@ int ffa_attention(ffa_plan_t* plan, const void* q, const void* k, const void* v,
 int ffa_attention_paged(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_pool, void* v_pool,
                         const int* page_table, int max_pages, int page_rows, void* out, float softmax_scale, int t,
                         const int* seq_lengths, int right_or_no_padding, float p, uint32_t* kept_mask, void* stream);
+
+/* ---- Attention of a tree of drafted tokens (speculative decoding).  No counterpart in the reference, which attends one
+ * token per call.
+ * q [batch, heads*groups, tokens, head_dim] (query head h*groups + g reads cache head h; groups = 1: as many query heads as
+ * cache heads), k and v [batch, heads, tokens, head_dim], out like q.  tree: one byte per pair of drafted tokens,
+ * [tokens, tokens], or [batch, tokens, tokens] with tree_per_sample != 0; row i sees drafted token j where it is nonzero
+ * (usually j's being i or an ancestor of i) and every visible cached row.  k and v are appended at rows row..row+tokens-1, where
+ * t, seq_lengths and right_or_no_padding mean what they mean in ffa_attention (with per-sample lengths a sample that lies above
+ * the bound t or has no room for its tokens is refused: FFA_STATUS_BAD_LENGTH, output zero, nothing appended).
+ * A query row that sees nothing is 0.  A token that a row does not see has no influence on it, whatever its values.
+ * Statistics and sums are fp32; fp16 and bf16 weights are rounded to the tensors' type before they meet V, and the result once.
+ * groups * tokens <= 1024.  page_table: NULL, or the paged caches of ffa_attention_paged.
+ * scratch: ffa_tree_scratch_bytes(plan, groups, tokens, t) bytes of device memory (may be 0), 16-byte aligned, used by this call
+ * only.  Like every call on a plan, calls are stream-ordered (the arrival counters are in the bound workspace). */
+int ffa_tree_scratch_bytes(const ffa_plan_t* plan, int groups, int tokens, int t, size_t* bytes);
+int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
+                       const unsigned char* tree, int tree_per_sample, int groups, int tokens, void* out, float softmax_scale,
+                       int t, const int* seq_lengths, int right_or_no_padding, const int* page_table, int max_pages,
+                       int page_rows, void* scratch, size_t scratch_bytes, void* stream);
+/* Keeps the accepted path of a tree: rows row + path[b, i] -> row + i of both caches, in place, i = 0, 1, ... up to the first
+ * negative entry.  path [batch, path_len] (device): strictly increasing tree indices (a node's ancestors come before it), so that no row is
+ * overwritten before it has moved; row = t, or seq_lengths[b].  A sample whose path is not increasing or leaves the cache is
+ * left as it was (FFA_STATUS_BAD_INDEX). */
+int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* path, int path_len, int t, const int* seq_lengths,
+                    const int* page_table, int max_pages, int page_rows, void* stream);
 
 /* The exact (p == 0, no per-sample lengths) decode step with NO caller-provided workspace and
  * no allocation of any kind inside the call.  It has no counterpart in the reference; it

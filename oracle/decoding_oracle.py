@@ -1,0 +1,75 @@
+"""Plain 64-bit definitions of the decoding strategies over the caches (drafted trees, eviction by accumulated weight, beam
+search), and the error bounds their kernels are held to.  CPU or GPU tensors; nothing here is fast."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+U = 2.0 ** -24   # half a step of fp32
+
+
+def half_step(dtype) -> float:
+    """Relative error of one rounding to `dtype`."""
+    return torch.finfo(dtype).eps / 2
+
+
+def tree_attention(q, k, v, k_cache, v_cache, tree, scale, rows, first=None):
+    """q [B, G*H, T, D]; k, v [B, H, T, D]; caches [B, H, L, D]; rows, first: per-sample lists.  Returns (out, bound) in float64:
+    the exact result of these inputs and how far a kernel of q's dtype may be from it."""
+    B, HG, T, D = q.shape
+    H = k.shape[1]
+    G = HG // H
+    out = torch.zeros(B, HG, T, D, dtype=torch.float64, device=q.device)
+    bound = torch.zeros_like(out)
+    for b in range(B):
+        n, lo = int(rows[b]), int(first[b]) if first is not None else 0
+        see = tree[b] if tree.dim() == 3 else tree
+        see = torch.cat([torch.ones(T, n - lo, dtype=torch.bool, device=q.device), see.bool()], 1)
+        for h in range(H):
+            keys = torch.cat([k_cache[b, h, lo:n], k[b, h]]).double()
+            vals = torch.cat([v_cache[b, h, lo:n], v[b, h]]).double()
+            for g in range(G):
+                x = q[b, h * G + g].double()
+                s = torch.where(see, (x @ keys.T) * scale, -math.inf)
+                m = s.amax(-1, keepdim=True)
+                p = torch.where(see, (s - torch.where(m == -math.inf, 0.0, m)).exp(), 0.0)
+                total = p.sum(-1, keepdim=True)
+                p = torch.where(total > 0, p / total, 0.0)
+                # a token that a row does not see has no part in it, whatever its values: 0 * inf is not formed
+                o = torch.stack([p[t][see[t]] @ vals[see[t]] for t in range(T)])
+                a = torch.stack([p[t][see[t]] @ vals[see[t]].abs() for t in range(T)])
+                out[b, h * G + g] = o
+                # dot product: D products and sums in fp32, one product with the scale; exp: its argument's rounding and two more steps
+                mag = torch.where(see, (x.abs() @ keys.abs().T) * abs(scale), 0.0)
+                ds = (D + 2) * U * mag.nan_to_num(0, 0, 0).amax(-1, keepdim=True)
+                smax = torch.where(see, s.abs(), 0.0).nan_to_num(0, 0, 0).amax(-1, keepdim=True)
+                dp = ds + 4 * U * (1 + smax)
+                rel = 2 * dp + (n - lo + T + 8) * U
+                err = rel * a
+                if q.dtype != torch.float32:
+                    err = err + half_step(q.dtype) * a            # weights rounded to the tensors' type
+                    if q.dtype == torch.float16:                   # weights below fp16's normal range: half its smallest step each
+                        err = err + 2.0 ** -25 * torch.stack([vals[see[t]].abs().sum(0) for t in range(T)])
+                bound[b, h * G + g] = err + half_step(q.dtype) * (o.abs() + err) + 1e-30
+    return out, bound
+
+
+def tree_accept(cache, path, rows):
+    """cache [B, H, L, D] -> a copy with rows n + path[b][i] at n + i."""
+    out = cache.clone()
+    for b, p in enumerate(path):
+        for i, j in enumerate(p):
+            out[b, :, rows[b] + i] = cache[b, :, rows[b] + j]
+    return out
+
+
+def assert_within(got, want, bound, what=""):
+    """Element by element; infinities and NaN have to be the same."""
+    got = got.double()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got), fin), f"{what}: finite values differ"
+    assert torch.equal(got[~fin].nan_to_num(7.0, 1e300, -1e300), want[~fin].nan_to_num(7.0, 1e300, -1e300)), f"{what}: infinities differ"
+    err = (got - want).abs()[fin]
+    over = err > bound[fin]
+    assert not over.any(), f"{what}: {int(over.sum())} of {over.numel()} off, worst {(err / bound[fin]).max().item():.2f} x the bound"

@@ -1,0 +1,312 @@
+"""Attention of a tree of drafted tokens over a cache, and the acceptance of a path, against their 64-bit definitions."""
+import pytest
+import torch
+
+from oracle import decoding_oracle as D64
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def random_tree(T, g, B=None):
+    def one():
+        see = torch.zeros(T, T, dtype=torch.bool)
+        for j in range(T):
+            if j:
+                see[j] = see[int(torch.randint(0, j, (1,), generator=g))]
+            see[j, j] = True
+        return see
+    return one() if B is None else torch.stack([one() for _ in range(B)])
+
+
+def setup(dt, B, H, G, D, n, T, L=None, seed=0, per_sample=True):
+    from fastforwardattention_b200 import FastForwardAttn
+
+    g = torch.Generator().manual_seed(seed)
+    L = L or n + T + 5
+    r = lambda *s: torch.randn(*s, generator=g).to(dt).cuda()
+    kc, vc = r(B, H, L, D), r(B, H, L, D)
+    q, k, v = r(B, H * G, T, D), r(B, H, T, D), r(B, H, T, D)
+    tree = random_tree(T, g, B if per_sample else None).cuda()
+    return FastForwardAttn.adopt(kc, vc), kc, vc, q, k, v, tree
+
+
+def check(ffa, kc, vc, q, k, v, tree, rows, call, first=None, what=""):
+    kb, vb = kc.clone(), vc.clone()
+    want, bound = D64.tree_attention(q, k, v, kb, vb, tree, q.shape[-1] ** -0.5, rows, first)
+    out = call()
+    D64.assert_within(out, want, bound, what)
+    T = k.shape[2]
+    for b, n in enumerate(rows):
+        kb[b, :, n:n + T], vb[b, :, n:n + T] = k[b], v[b]
+    assert torch.equal(kb, kc) and torch.equal(vb, vc), what + ": the caches hold other rows than the appended ones"
+    assert ffa.device_status() == 0
+    return out
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("G,T,n", [(1, 1, 0), (1, 1, 1), (1, 3, 200), (1, 8, 63), (2, 5, 64), (1, 33, 129), (4, 33, 65), (1, 100, 31), (8, 40, 300),
+                                   (1, 64, 64), (1, 129, 7)])
+def test_against_definition(dt, D, G, T, n):
+    ffa, kc, vc, q, k, v, tree = setup(dt, 2, 3, G, D, n, T, seed=T * 1000 + n, per_sample=T % 2 == 1)
+    check(ffa, kc, vc, q, k, v, tree, [n, n], lambda: ffa.tree_attention(q, k, v, tree, D ** -0.5, n), what=f"{dt} {D} {G} {T} {n}")
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("T,G", [(1, 1), (7, 1), (20, 2), (64, 4)])
+def test_long_cache_is_split_over_ctas(dt, T, G):
+    n, D = 4099, 128
+    ffa, kc, vc, q, k, v, tree = setup(dt, 1, 2, G, D, n, T, seed=T)
+    out = check(ffa, kc, vc, q, k, v, tree, [n], lambda: ffa.tree_attention(q, k, v, tree, D ** -0.5, n))
+    for _ in range(3):   # the splits are merged in a fixed order, and the arrival counters are ready again
+        assert torch.equal(out, ffa.tree_attention(q, k, v, tree, D ** -0.5, n))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_per_sample_lengths_and_bound(dt):
+    B, D, T, n = 6, 64, 13, 700
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, 2, 1, D, n, T, seed=5)
+    rows = [0, 1, 64, 333, 699, 700]
+    sl = torch.tensor(rows, dtype=torch.int32, device="cuda")
+    for bound in (-1, n, n + 3):
+        check(ffa, kc, vc, q, k, v, tree, rows, lambda: ffa.tree_attention_per_sample(q, k, v, tree, D ** -0.5, sl, max_row=bound))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_left_padding(dt):
+    B, D, T, n = 5, 128, 9, 257
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, 2, 2, D, n, T, seed=6)
+    first = [0, 1, 64, 200, 257]
+    for b, lo in enumerate(first):   # what the padding rows hold never matters
+        kc[b, :, :lo], vc[b, :, :lo] = float("nan"), float("inf")
+    kb, vb = kc.clone(), vc.clone()
+    want, bound = D64.tree_attention(q, k, v, kb, vb, tree, D ** -0.5, [n] * B, first)
+    out = ffa.tree_attention(q, k, v, tree, D ** -0.5, n, seq_lengths=torch.tensor(first, dtype=torch.int32, device="cuda"))
+    D64.assert_within(out, want, bound)
+    assert ffa.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("n,T", [(0, 6), (130, 6), (130, 70), (4000, 20)])
+def test_hidden_and_stale_values_have_no_influence(dt, n, T):
+    """NaN and infinities in cache rows behind the last one, and in drafted tokens that a row does not see."""
+    D = 64
+    ffa, kc, vc, q, k, v, tree = setup(dt, 1, 2, 1, D, n, T, seed=n + T, L=n + T + 90)
+    kc[:, :, n:], vc[:, :, n:] = float("nan"), float("inf")
+    bad = T - 2
+    k[:, :, bad], v[:, 0, bad] = float("nan"), float("inf")
+    v[:, 1, bad] = float("nan")
+    tree[:, :, bad] = False
+    want, bound = D64.tree_attention(q, k, v, kc, vc, tree, D ** -0.5, [n])
+    assert torch.isfinite(want).all()
+    D64.assert_within(ffa.tree_attention(q, k, v, tree, D ** -0.5, n), want, bound)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_a_visible_infinity_reaches_the_rows_that_see_it_and_no_others(dt):
+    D, T, n = 64, 12, 100
+    ffa, kc, vc, q, k, v, tree = setup(dt, 1, 1, 1, D, n, T, seed=9)
+    v[0, 0, 3, 5], v[0, 0, 4, 6] = float("inf"), float("nan")
+    want, bound = D64.tree_attention(q, k, v, kc, vc, tree, D ** -0.5, [n])
+    assert not torch.isfinite(want).all() and torch.isfinite(want[0, 0, 0]).all()
+    D64.assert_within(ffa.tree_attention(q, k, v, tree, D ** -0.5, n), want, bound)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("T", [4, 40, 140])
+def test_rows_that_see_nothing_are_zero(dt, T):
+    D = 128
+    ffa, kc, vc, q, k, v, tree = setup(dt, 2, 1, 1, D, 0, T, seed=11)
+    tree[0] = False
+    tree[1, 1] = False
+    out = check(ffa, kc, vc, q, k, v, tree, [0, 0], lambda: ffa.tree_attention(q, k, v, tree, D ** -0.5, 0))
+    assert (out[0] == 0).all() and (out[1, :, 1] == 0).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_scores_that_grow_along_the_cache(dt):
+    """The running maximum moves by far more than any exponent range, upwards in every tile; and once downwards."""
+    D, n, T = 64, 640, 17
+    for sign in (1.0, -1.0):
+        ffa, kc, vc, q, k, v, tree = setup(dt, 1, 2, 1, D, n, T, seed=13)
+        q[:] = 1.0
+        ramp = torch.linspace(-8, 8, n, device="cuda") * sign
+        kc[:, :, :n] = ramp[:, None].to(dt)
+        check(ffa, kc, vc, q, k, v, tree, [n], lambda: ffa.tree_attention(q, k, v, tree, D ** -0.5, n))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_strided_inputs_out_argument_and_other_stream(dt):
+    B, H, D, T, n = 2, 4, 64, 11, 90
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, H, 1, D, n, T, seed=17)
+    wide = torch.randn(B, T, 3, H, D, device="cuda").to(dt)   # a fused projection's output
+    q, k, v = (wide[:, :, i].transpose(1, 2) for i in range(3))
+    big = torch.zeros(B, 2 * T, 2 * T, dtype=torch.bool, device="cuda")
+    big[:, ::2, 1::2] = tree
+    out = torch.full((B, H, T, D), 7.0, dtype=dt, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = check(ffa, kc, vc, q, k, v, big[:, ::2, 1::2], [n] * B,
+                    lambda: ffa.tree_attention(q, k, v, big[:, ::2, 1::2], D ** -0.5, n, out=out))
+    side.synchronize()
+    assert got.data_ptr() == out.data_ptr()
+    assert torch.equal(ffa.tree_attention(q, k, v, tree.to(torch.uint8), D ** -0.5, n), out)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_captured_and_replayed_with_lengths_on_the_device(dt):
+    B, H, D, T, n = 2, 2, 128, 21, 2500
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, H, 1, D, n, T, L=n + 4 * T, seed=19)
+    rows = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    path = torch.tensor([[0, 2, 5], [1, -1, -1]], dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    ffa.tree_attention_per_sample(q, k, v, tree, D ** -0.5, rows, out=out, max_row=n + 3 * T)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ffa.tree_attention_per_sample(q, k, v, tree, D ** -0.5, rows, out=out, max_row=n + 3 * T)
+        ffa.tree_accept_per_sample(path, rows)
+        rows += (path >= 0).sum(1, dtype=torch.int32)
+    now = [n, n]
+    for _ in range(3):
+        for x in (q, k, v):
+            x.normal_()
+        kb, vb = kc.clone(), vc.clone()
+        want, bound = D64.tree_attention(q, k, v, kb, vb, tree, D ** -0.5, now)
+        graph.replay()
+        D64.assert_within(out, want, bound)
+        for cache, new in ((kb, k), (vb, v)):
+            for b, m in enumerate(now):
+                cache[b, :, m:m + T] = new[b]
+            cache.copy_(D64.tree_accept(cache, [[0, 2, 5], [1]], now))
+        assert torch.equal(kb, kc) and torch.equal(vb, vc)
+        now = [now[0] + 3, now[1] + 1]
+    assert rows.tolist() == now and ffa.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_accept_moves_the_path_to_the_front(dt, D):
+    from fastforwardattention_b200 import FastForwardAttn
+
+    B, H, L, n = 4, 3, 120, 37
+    kc, vc = (torch.randn(B, H, L, D, device="cuda").to(dt) for _ in range(2))
+    ffa = FastForwardAttn.adopt(kc, vc)
+    paths = [list(range(1, 40, 2)), [], [0, 1, 2, 50], [L - n - 6]]
+    flat = torch.full((B, 20), -1, dtype=torch.int32)
+    for b, p in enumerate(paths):
+        flat[b, : len(p)] = torch.tensor(p, dtype=torch.int32)
+    rows = [n, n + 1, n + 2, n + 5]
+    want = [D64.tree_accept(c, paths, rows) for c in (kc, vc)]
+    ffa.tree_accept_per_sample(flat.cuda(), torch.tensor(rows, dtype=torch.int32, device="cuda"))
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1]) and ffa.device_status() == 0
+    want = [D64.tree_accept(c, [[2, 3]] * B, [n] * B) for c in (kc, vc)]
+    ffa.tree_accept(torch.tensor([[2, 3]] * B, dtype=torch.int32, device="cuda"), n)
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+    ffa.tree_accept(torch.empty(B, 0, dtype=torch.int32, device="cuda"), n)
+    assert torch.equal(kc, want[0])
+
+
+def test_what_the_device_refuses():
+    """Lengths and paths that only the device sees: reported, zeros out, nothing appended or moved for that sample; the others go on."""
+    dt, B, D, T, n = torch.float16, 4, 64, 6, 50
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, 2, 1, D, n, T, L=64, seed=23)
+    kb, vb = kc.clone(), vc.clone()
+    rows = torch.tensor([n, 59, -1, 10], dtype=torch.int32, device="cuda")   # 59 + 6 > 64
+    out = ffa.tree_attention_per_sample(q, k, v, tree, D ** -0.5, rows)
+    assert ffa.device_status() == 2
+    want, bound = D64.tree_attention(q, k, v, kb, vb, tree, D ** -0.5, [n, 0, 0, 10])
+    for b in (0, 3):
+        D64.assert_within(out[b], want[b], bound[b])
+    assert (out[1:3] == 0).all() and torch.equal(kc[1:3], kb[1:3]) and torch.equal(vc[1:3], vb[1:3])
+    ffa.tree_attention_per_sample(q, k, v, tree, D ** -0.5, rows.clamp(0, 40), max_row=30)   # above the stated bound
+    assert ffa.device_status() == 2
+    kb = kc.clone()
+    ffa.tree_accept_per_sample(torch.tensor([[0, 2], [2, 1], [3, 3], [13, 14]], dtype=torch.int32, device="cuda"),
+                               torch.tensor([20, 20, 20, 50], dtype=torch.int32, device="cuda"))
+    assert ffa.device_status() == 4
+    assert torch.equal(kc[1:], kb[1:]) and torch.equal(kc[0], D64.tree_accept(kb, [[0, 2], [], [], []], [20] * 4)[0])
+
+
+def test_refusals_from_python():
+    dt, B, H, D, T, n = torch.bfloat16, 2, 2, 64, 4, 20
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, H, 1, D, n, T, L=32, seed=29)
+    s = D ** -0.5
+    for bad, match in [((q.float(), k, v, tree, s, n), "dtype"), ((q[:, :1], k, v, tree, s, n), "multiple"), ((q, k[:, :, :2], v, tree, s, n), "k must be"),
+                       ((q, k, v.cpu(), tree, s, n), "v must be"), ((q, k, v, tree.float(), s, n), "tree"), ((q, k, v, tree[:, :2], s, n), "tree"),
+                       ((q, k, v, tree, s, 32), "outside"), ((q, k, v, tree, s, 29), "exceeds the cache"), ((q, k, v, tree, s, -1), "outside")]:
+        with pytest.raises(RuntimeError, match=match):
+            ffa.tree_attention(*bad)
+    with pytest.raises(RuntimeError, match="seq_lengths"):
+        ffa.tree_attention_per_sample(q, k, v, tree, s, torch.zeros(B, dtype=torch.int64, device="cuda"))
+    with pytest.raises(RuntimeError, match="out must"):
+        ffa.tree_attention(q, k, v, tree, s, n, out=torch.empty(B, H, T, D, device="cuda"))
+    many = torch.ones(1025, 1025, dtype=torch.bool, device="cuda")
+    with pytest.raises(RuntimeError, match="1024"):
+        ffa.tree_attention(torch.zeros(B, H, 1025, D, dtype=dt, device="cuda"), k, v, many, s, n)
+    with pytest.raises(RuntimeError, match="path"):
+        ffa.tree_accept(torch.zeros(B, 2, dtype=torch.int64, device="cuda"), n)
+    assert ffa.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_paged_sequences_draft_and_accept(dt):
+    from fastforwardattention_b200 import PagedFastForwardAttn, PagePool
+
+    B, H, D, T = 3, 2, 128, 24
+    lens = [130, 250, 1]
+    pool = PagePool(16, H, D, dt, "cuda", page_rows=128)
+    pool.k.fill_(float("nan")), pool.v.fill_(float("nan"))
+    K, V = (torch.randn(B, H, 256, D, device="cuda").to(dt) for _ in range(2))
+    seqs = PagedFastForwardAttn(pool, K, V, 512, lengths=lens)
+    kc, vc = (torch.zeros(B, H, 512, D, dtype=dt, device="cuda") for _ in range(2))
+    for b, n in enumerate(lens):
+        kc[b, :, :n], vc[b, :, :n] = K[b, :, :n], V[b, :, :n]
+    g = torch.Generator().manual_seed(31)
+    now = list(lens)
+    for step in range(3):
+        q, k, v = (torch.randn(B, h, T, D, generator=g).to(dt).cuda() for h in (2 * H, H, H))
+        tree = random_tree(T, g, B).cuda()
+        want, bound = D64.tree_attention(q, k, v, kc, vc, tree, D ** -0.5, now)
+        D64.assert_within(seqs.tree_attention(q, k, v, tree, D ** -0.5), want, bound, f"step {step}")
+        path = [[0, 3, 7, 20], [step], list(range(step))]
+        seqs.tree_accept(path)
+        for b, p in enumerate(path):
+            for i, j in enumerate(p):
+                kc[b, :, now[b] + i], vc[b, :, now[b] + i] = k[b, :, j], v[b, :, j]
+        now = [n + len(p) for n, p in zip(now, path)]
+        assert seqs.lengths == now == seqs.rows.tolist()
+    q, k, v = (torch.randn(B, H, 1, D, generator=g).to(dt).cuda() for _ in range(3))
+    one = torch.ones(1, 1, dtype=torch.bool, device="cuda")
+    want, bound = D64.tree_attention(q, k, v, kc, vc, one, D ** -0.5, now)
+    D64.assert_within(seqs.attention(q, k, v, D ** -0.5)[:, :, None], want, bound, "one-token step")
+    assert seqs.engine.device_status() == 0
+    for bad in ([[0], [0]], [[1, 0], [], []], [[-1], [], []], [[300], [], []]):
+        with pytest.raises(ValueError):
+            seqs.tree_accept(bad)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_drafting_agrees_with_one_token_steps(dt):
+    """Speculative decoding as it is used: a tree over the cache, its accepted path kept, then a one-token step; the one-token steps
+    over the same path give the same outputs."""
+    from fastforwardattention_b200 import FastForwardAttn
+
+    B, H, D, n, T = 2, 4, 64, 300, 10
+    g = torch.Generator().manual_seed(37)
+    K, V = (torch.randn(B, H, n, D, generator=g).to(dt).cuda() for _ in range(2))
+    a, c = FastForwardAttn(K, V, n + 32, False), FastForwardAttn(K, V, n + 32, False)
+    tree = random_tree(T, g)
+    path = tree[T - 1].nonzero().flatten().tolist()
+    tree = tree.cuda()
+    q, k, v = (torch.randn(B, H, T, D, generator=g).to(dt).cuda() for _ in range(3))
+    _, bound = D64.tree_attention(q, k, v, *a.get_cache(), tree, D ** -0.5, [n] * B)
+    out = a.tree_attention(q, k, v, tree, D ** -0.5, n)
+    a.tree_accept(torch.tensor([path] * B, dtype=torch.int32, device="cuda"), n)
+    for i, j in enumerate(path):
+        step = c.attention(q[:, :, j].contiguous(), k[:, :, j].contiguous(), v[:, :, j].contiguous(), D ** -0.5, n + i, 0)
+        assert ((step.double() - out[:, :, j].double()).abs() <= 2 * bound[:, :, j]).all()
+    for x, y in zip(a.get_cache(), c.get_cache()):
+        assert torch.equal(x[:, :, : n + len(path)], y[:, :, : n + len(path)])
