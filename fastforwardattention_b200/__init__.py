@@ -11,7 +11,8 @@ from __future__ import annotations
 
 import importlib
 
-__all__ = ["FastForwardAttn", "ShardedFastForwardAttn", "GraphedStep", "GraphedHostStep", "GraphedLayers", "PagePool", "PagedFastForwardAttn", "launch_count"]
+__all__ = ["FastForwardAttn", "ShardedFastForwardAttn", "GraphedStep", "GraphedHostStep", "GraphedLayers", "PagePool", "PagedFastForwardAttn", "EvictingFastForwardAttn", "beam_select",
+           "launch_count"]
 
 
 def _extension():
@@ -27,8 +28,12 @@ def _extension():
 def __getattr__(name):
     if name == "FastForwardAttn":
         return _extension().FastForwardAttn
-    if name == "launch_count":
-        return _extension().launch_count
+    if name in ("launch_count", "beam_select"):
+        return getattr(_extension(), name)
+    if name == "EvictingFastForwardAttn":
+        from .evicting import EvictingFastForwardAttn
+
+        return EvictingFastForwardAttn
     if name in ("PagePool", "PagedFastForwardAttn"):
         from . import paged
 

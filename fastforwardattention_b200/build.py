@@ -30,6 +30,9 @@ COMMON_HEADERS = ["ffa_internal.h", "ffa_device_common.cuh", "ffa_launch.cuh"]
 CUDA_SOURCES = {
     "ffa_decode_kernels.cu": [*COMMON_HEADERS, "ffa_stream_kernel.cuh", "ffa_prune_kernels.cuh", "ffa_prune_stream_kernel.cuh"],
     "ffa_tree_kernels.cu": [*COMMON_HEADERS, "ffa_tree_kernel.cuh"],
+    "ffa_evict_kernels.cu": COMMON_HEADERS,
+    "ffa_beam_kernels.cu": COMMON_HEADERS,
+    "ffa_strategies_api.cu": ["ffa_internal.h", "ffa_plan.h", API_HEADER],
     "ffa_tree_api.cu": ["ffa_internal.h", "ffa_plan.h", API_HEADER],
     "ffa_c_api.cu": ["ffa_internal.h", "ffa_plan.h", API_HEADER],
     "ffa_no_alloc.cu": ["ffa_internal.h", API_HEADER],

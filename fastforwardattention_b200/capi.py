@@ -19,7 +19,8 @@ SYMBOLS = ["ffa_cache_bytes", "ffa_cache_init", "ffa_plan_create", "ffa_plan_des
            "ffa_plan_get_prune_launch", "ffa_plan_get_prune_path", "ffa_cache_copy", "ffa_attention_paged", "ffa_peer_gather_bytes",
            "ffa_peer_mem_alloc", "ffa_peer_mem_open", "ffa_peer_mem_close", "ffa_peer_mem_free", "ffa_peer_gather_attach",
            "ffa_peer_gather", "ffa_plan_set_cluster_merge", "ffa_peer_push_target",
-           "ffa_tree_scratch_bytes", "ffa_tree_attention", "ffa_tree_accept"]
+           "ffa_tree_scratch_bytes", "ffa_tree_attention", "ffa_tree_accept", "ffa_attention_accumulate", "ffa_evict", "ffa_beam_select",
+           "ffa_cache_reorder"]
 
 
 class Launch(C.Structure):
@@ -79,6 +80,10 @@ def lib() -> C.CDLL:
         L.ffa_tree_scratch_bytes.argtypes = [vp, i, i, i, C.POINTER(sz)]
         L.ffa_tree_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, vp, f, i, vp, i, vp, i, i, vp, sz, vp]
         L.ffa_tree_accept.argtypes = [vp, vp, vp, vp, i, i, vp, vp, i, i, vp]
+        L.ffa_attention_accumulate.argtypes = [vp, vp, vp, vp, vp, vp, vp, f, i, vp, vp, vp, vp, vp]
+        L.ffa_evict.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, vp, vp]
+        L.ffa_beam_select.argtypes = [i, i, i, i, C.c_longlong, vp, vp, vp, i, i, vp, vp, vp, vp]
+        L.ffa_cache_reorder.argtypes = [vp, vp, vp, vp, i, i, i, vp]
         L.ffa_launch_count.restype = C.c_ulonglong
         L.ffa_last_error.restype = C.c_char_p
         _lib = L

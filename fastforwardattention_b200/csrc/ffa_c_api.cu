@@ -423,6 +423,7 @@ int ffa_plan_create(int dtype, int batch, int heads, int head_dim, int max_len, 
     int r = 0;
     if (e == cudaSuccess) r = ffa_k_prepare(dtype, head_dim, smem_cta);
     if (e == cudaSuccess && r == 0) r = ffa_k_tree_prepare(dtype, head_dim);
+    if (e == cudaSuccess && r == 0) r = ffa_k_evict_prepare(smem_cta);
     cudaSetDevice(prev);
     if (e != cudaSuccess) return cuda_fail(e, "device attribute query");
     if (r != 0) return cuda_fail(r, "kernel preparation (is this an sm_100a device?)");
@@ -569,11 +570,17 @@ struct PageArgs {
     const int* table = nullptr;
     int max_pages = 0, page_rows = 0;
 };
+// what an accumulating step adds to a decode step
+struct WeighArgs {
+    float* weights = nullptr;
+    int* positions = nullptr;
+    const int* seen = nullptr;
+};
 
 // One decode step on contiguous caches (pages.table == nullptr) or page pools.
 int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache, void* out,
              float softmax_scale, int t, const int* seq_lengths, int right_or_no_padding, float p, uint32_t* kept_mask,
-             const PageArgs& pages, void* stream)
+             const PageArgs& pages, void* stream, const WeighArgs& weigh = WeighArgs{})
 {
     if (plan == nullptr) return fail(FFA_ERR_ARG, "null plan");
     if (plan->offline) return fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
@@ -586,7 +593,8 @@ int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void
         return fail(FFA_ERR_ARG, "left padding (right_or_no_padding = 0) needs seq_lengths");
     if (plan->ws == nullptr) return fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
     const bool paged = pages.table != nullptr;
-    const bool twopass = p > 0.f || plan->mode == FFA_MODE_ROUND_LIKE_TORCH;
+    const bool weighs = weigh.weights != nullptr;   // always in the exact mode's arithmetic
+    const bool twopass = !weighs && (p > 0.f || plan->mode == FFA_MODE_ROUND_LIKE_TORCH);
     const int cap = t;   // rows the unit list covers: every sample is at row t, or (per-sample lengths) at a row no greater than the bound t
     FfaStepParams P;
     std::memset(&P, 0, sizeof(P));
@@ -599,6 +607,9 @@ int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void
     P.scores = plan->scores, P.score_stride = score_stride(plan->Lmax);
     P.kept_mask = kept_mask, P.mask_words = (plan->Lmax + 31) / 32;
     P.page_table = pages.table, P.max_pages = pages.max_pages, P.page_rows = pages.page_rows;
+    P.weights = weigh.weights, P.positions = weigh.positions, P.seen = weigh.seen;
+    if (weighs && plan->scores == nullptr)
+        return fail(FFA_ERR_WORKSPACE, "accumulating steps keep their scores in the workspace: bind one sized with with_scores = 1");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
 
     // p > 0 / torch rounding.  Small steps: the cluster kernel (scores stay in shared memory, nothing but the
@@ -624,6 +635,14 @@ int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void
         return fail(FFA_ERR_WORKSPACE, "this shape needs the streaming pruning kernel: bind a workspace sized with with_scores = 1");
 
     ffa_launch_t L;
+    // accumulating steps merge split pairs through global memory, whose last arriver adds the weights: the cut is the one of
+    // a plan without the cluster merge
+    ffa_plan without_clusters;
+    if (weighs) {
+        without_clusters = *plan;
+        without_clusters.cluster_merge = 0;
+        plan = &without_clusters;
+    }
     // the streaming kernel never lets a tile straddle a page: tiles are powers of two that divide it
     int r = fit_launch(plan, cap, twopass ? 1 : 2, &L, /*pow2_tiles=*/paged);
     if (r != FFA_OK) return r;
@@ -632,7 +651,7 @@ int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void
     P.units_per_bh = cap / L.tile_rows + 1;
     P.parts_per_bh = L.parts_per_bh;
     if (!twopass) {
-        if (plan->push_gathered != nullptr && plan->peer_world > 1 && !paged) {
+        if (plan->push_gathered != nullptr && plan->peer_world > 1 && !paged && !weighs) {
             // the kernel's epilogue is the push phase of the output all-gather
             for (int r = 0; r < plan->peer_world; ++r) P.push_peer[r] = plan->peer_buf[r];
             P.push_gathered = plan->push_gathered, P.push_half_bytes = peer_half_bytes(plan, plan->peer_world);
@@ -680,6 +699,16 @@ int ffa_attention_paged(ffa_plan_t* plan, const void* q, const void* k, const vo
     pages.table = page_table, pages.max_pages = max_pages, pages.page_rows = page_rows;
     return run_step(plan, q, k, v, k_pool, v_pool, out, softmax_scale, t, seq_lengths, right_or_no_padding, p, kept_mask, pages,
                     stream);
+}
+
+int ffa_attention_accumulate(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache, void* out,
+                             float softmax_scale, int t, const int* seq_lengths, float* weights, int* positions, const int* seen, void* stream)
+{
+    if (plan == nullptr) return fail(FFA_ERR_ARG, "null plan");
+    if (weights == nullptr) return fail(FFA_ERR_ARG, "null weights");
+    WeighArgs w;
+    w.weights = weights, w.positions = positions, w.seen = seen;
+    return run_step(plan, q, k, v, k_cache, v_cache, out, softmax_scale, t, seq_lengths, 1, 0.f, nullptr, PageArgs{}, stream, w);
 }
 
 int ffa_selftest_wait_timeout(ffa_plan_t* plan, unsigned int limit_ms, void* stream)

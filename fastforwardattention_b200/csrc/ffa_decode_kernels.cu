@@ -8,7 +8,7 @@
 // runs, one per CTA of a persistent grid, so all SMs stream from HBM whatever the batch*head
 // count and the sequence length is bounded by memory only.
 //
-//   ffa_stream_kernel<T, DH>              p == 0: K and V tiles through a bulk-copy ring,
+//   ffa_stream_kernel<T, DH, kWeigh>      p == 0: K and V tiles through a bulk-copy ring,
 //                                         online softmax, cross-CTA merge by the CTA that
 //                                         arrives last (no waiting), k/v append fused
 //   ffa_prune_stream_kernel<T, DH>        p > 0 on large steps, one persistent launch: K tiles
@@ -138,7 +138,9 @@ int ffa_k_prepare(int dtype, int head_dim, int max_smem_bytes)
             if (err != cudaSuccess) return err;
             return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem_bytes - (int)a.sharedSizeBytes);
         };
-        cudaError_t e = raise_limit(reinterpret_cast<const void*>(ffa_stream_kernel<T, DH>));
+        cudaError_t e = raise_limit(reinterpret_cast<const void*>(ffa_stream_kernel<T, DH, false>));
+        if (e != cudaSuccess) return (int)e;
+        e = raise_limit(reinterpret_cast<const void*>(ffa_stream_kernel<T, DH, true>));
         if (e != cudaSuccess) return (int)e;
         e = raise_limit(reinterpret_cast<const void*>(ffa_prune_stream_kernel<T, DH>));
         if (e != cudaSuccess) return (int)e;
@@ -181,15 +183,17 @@ int ffa_k_decode_onepass(int dtype, int head_dim, const FfaStepParams& P, int th
         constexpr int DH = decltype(dh)::value;
         // rows the step streams: at most t of every pair (per-sample lengths: t is their bound)
         const bool overlap = 2.0 * P.B * P.H * P.t * DH * sizeof(T) < kPdlBelowBytes;
+        if (P.weights != nullptr)
+            return (int)launch_pdl(ffa_stream_kernel<T, DH, true>, P.grid, threads, smem, 0, overlap, stream, P);
         if (P.cluster > 1) {   // the CTAs that share a (batch, head) as one thread-block cluster
-            if (launch_pdl(ffa_stream_kernel<T, DH>, P.grid, threads, smem, P.cluster, overlap, stream, P) == cudaSuccess) return 0;
+            if (launch_pdl(ffa_stream_kernel<T, DH, false>, P.grid, threads, smem, P.cluster, overlap, stream, P) == cudaSuccess) return 0;
             // a cluster shape this device cannot co-schedule: the same cut runs without clusters,
             // the parts merging through global memory
             (void)cudaGetLastError();
         }
         FfaStepParams Q = P;
         Q.cluster = 0;
-        return (int)launch_pdl(ffa_stream_kernel<T, DH>, Q.grid, threads, smem, 0, overlap, stream, Q);
+        return (int)launch_pdl(ffa_stream_kernel<T, DH, false>, Q.grid, threads, smem, 0, overlap, stream, Q);
     });
 }
 
@@ -207,7 +211,7 @@ int ffa_k_max_active_clusters(int dtype, int head_dim, int threads, int smem, in
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = (unsigned)cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
         cfg.attrs = &attr, cfg.numAttrs = 1;
-        return (int)cudaOccupancyMaxActiveClusters(clusters, ffa_stream_kernel<T, DH>, &cfg);
+        return (int)cudaOccupancyMaxActiveClusters(clusters, ffa_stream_kernel<T, DH, false>, &cfg);
     });
 }
 

@@ -42,6 +42,11 @@ struct FfaStepParams {
     void* push_gathered;    // [B][push_world * H][Dh]: this rank's own result tensor
     size_t push_half_bytes;
     int push_world, push_rank;
+    // Accumulated attention weights (ffa_attention_accumulate; the accumulating kernel only): weights[pair, r] += p[r] for the
+    // cached rows that are attended, weights[pair, new row] = p[new], positions[pair, new row] = seen[sample]
+    float* weights;     // [B*H, Lmax]
+    int* positions;     // [B*H, Lmax] or null
+    const int* seen;    // [B] or null: the new row's index
 };
 
 // 32-bit words of the 256-byte tail of a staging buffer: arrival flags (one per peer), the step counter, the ticket that
@@ -67,7 +72,7 @@ struct FfaPeerGatherParams {
 int ffa_k_prepare(int dtype, int head_dim, int max_smem_bytes);
 int ffa_k_cache_init(int dtype, int BH, int prompt_len, int src_len, int max_len, int head_dim, const void* k_src,
                      const void* v_src, void* k_cache, void* v_cache, int sms, cudaStream_t stream);
-// p == 0, exact mode: one launch.
+// p == 0, exact mode: one launch (accumulating the attention weights when P.weights is set).
 int ffa_k_decode_onepass(int dtype, int head_dim, const FfaStepParams& P, int threads, int smem, cudaStream_t stream);
 // how many clusters of `cluster` CTAs of the one-pass kernel the device keeps resident at once
 int ffa_k_max_active_clusters(int dtype, int head_dim, int threads, int smem, int cluster, int* clusters);
@@ -128,3 +133,43 @@ int ffa_k_tree_smem(int dtype, int head_dim, int rows);
 int ffa_k_tree_prepare(int dtype, int head_dim);
 int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaStream_t stream);
 int ffa_k_tree_accept(const FfaAcceptParams& P, cudaStream_t stream);
+
+// Eviction down to a budget of rows per pair (ffa_evict).
+struct FfaEvictParams {
+    void* k_cache;      // [B*H, Lmax, Dh]
+    void* v_cache;
+    float* weights;     // [B*H, Lmax]
+    int* positions;     // [B*H, Lmax]
+    const int* rows;    // [B] rows in use of every sample
+    int* kept;          // [B*H, keep]: the row that each row was before the call, -1 behind the sample's rows
+    int B, H, Lmax, max_rows, keep, recent, first, row_bytes;
+    int* status;
+};
+int ffa_k_evict_smem(int max_rows);
+int ffa_k_evict_prepare(int max_smem);
+int ffa_k_evict(const FfaEvictParams& P, int smem, cudaStream_t stream);
+
+// Selection over beams and vocabulary (ffa_beam_select).
+struct FfaBeamParams {
+    const void* logits;              // [batch, beams, vocab], rows row_stride elements apart
+    const float* scores;             // [batch, beams]
+    const unsigned char* finished;   // [batch, beams] or null
+    float* out_scores;               // [batch, num]
+    int* out_parents;
+    int* out_tokens;
+    long long row_stride;
+    int batch, beams, vocab, num, pad_token;
+};
+constexpr int kMaxBeams = 32;
+constexpr int kMaxBeamCandidates = 64;
+int ffa_k_beam_select(int dtype, const FfaBeamParams& P, cudaStream_t stream);
+// Reordering of the caches by parent beam (ffa_cache_reorder).
+struct FfaReorderParams {
+    void* k_cache;        // [groups * beams, H, Lmax, Dh]
+    void* v_cache;
+    const int* parents;   // [groups, beams]
+    int groups, beams, H, Lmax, first, rows, row_bytes;
+    int chunks;           // blocks per (group, head) and tensor (set by the launcher)
+    int* status;
+};
+int ffa_k_reorder(FfaReorderParams P, int sms, cudaStream_t stream);

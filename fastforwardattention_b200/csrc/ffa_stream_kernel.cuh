@@ -66,7 +66,10 @@ __device__ __forceinline__ void merge_partials(const FfaStepParams& P, uint32_t 
 // Warp 0 issues the copies (one elected lane); warps 1.. compute.  A lane group of LPR lanes
 // owns a row: 16-byte shared-memory reads, fp32 FMAs, butterfly sum.  Each group keeps its
 // own online-softmax state, so the row loop has no CTA-level synchronisation at all.
-template <typename T, int DH>
+// kWeigh: the step also accumulates every attended row's probability into P.weights.  A row's score goes to the score scratch as
+// it is computed (4 bytes a row, L2-resident); the CTA that completes a pair -- the one that owns it whole, or the last to
+// arrive -- reads the scores back once the pair's maximum and sum are known.  Runs without the cluster merge.
+template <typename T, int DH, bool kWeigh>
 // Register budget: 4 resident CTAs of 160 threads (or 2 of 288) need <= 96 registers per thread;
 // head_dim 80 keeps five vectors per lane in flight and is compiled for 2 CTAs of 160 threads.
 __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_stream_kernel(const FfaStepParams P)
@@ -229,7 +232,8 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
             // RB (four; two for head_dim 80) rows per lane group at a time: all shared-memory loads first, then the
             // packed fp32 FMAs (fma.rn.f32x2), four interleaved butterfly sums, one softmax
             // update.  FULL: every row of the batch exists (no predicates, no clamping).
-            auto batch = [&](auto full_tag, const unsigned char* ks, const unsigned char* vs, int base, int nrows) {
+            float* pair_scores = kWeigh ? P.scores + (size_t)bh * P.score_stride : nullptr;
+            auto batch = [&](auto full_tag, const unsigned char* ks, const unsigned char* vs, int base, int nrows, int first_row) {
                 constexpr bool FULL = decltype(full_tag)::value;
                 int rc[RB];
                 uint4 kraw[RB][VPL];
@@ -262,6 +266,11 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                     for (int uu = 0; uu < RB; ++uu) sc[uu] += __shfl_xor_sync(0xffffffffu, sc[uu], off);
 #pragma unroll
                 for (int uu = 0; uu < RB; ++uu) sc[uu] = (FULL || base + uu * NG + g < nrows) ? score_of(sc[uu]) : -CUDART_INF_F;
+                if constexpr (kWeigh) {
+#pragma unroll
+                    for (int uu = 0; uu < RB; ++uu)
+                        if (li == 0 && (FULL || base + uu * NG + g < nrows)) pair_scores[first_row + base + uu * NG + g] = sc[uu];
+                }
                 float m_new = m;
 #pragma unroll
                 for (int uu = 0; uu < RB; ++uu) m_new = fmaxf(m_new, sc[uu]);
@@ -313,8 +322,8 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                     const unsigned char* vs = ks + tile_bytes;
                     if (ready) {
                         int base = 0;
-                        for (; base + RB * NG <= nrows; base += RB * NG) batch(std::true_type{}, ks, vs, base, nrows);
-                        if (base < nrows) batch(std::false_type{}, ks, vs, base, nrows);
+                        for (; base + RB * NG <= nrows; base += RB * NG) batch(std::true_type{}, ks, vs, base, nrows, lo);
+                        if (base < nrows) batch(std::false_type{}, ks, vs, base, nrows, lo);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_empty + 8 * stage);
@@ -335,6 +344,7 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                 dot = group_sum<LPR>(dot);  // every group computes it; group 0 uses it
                 if (g == 0) {
                     const float st = score_of(dot);
+                    if (kWeigh && li == 0) pair_scores[sr.row] = st;
                     const float m_new = fmaxf(m, st);
                     const float corr = expo(m - m_new), pr = expo(st - m_new);
                     m = m_new;
@@ -428,6 +438,30 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                     merge_partials<T, DH, kPrecise>(P, push_seq, bh, P.partials + (size_t)(c_first + bh) * (DH + 2), count, outp, ctid, nct);
                     if (ctid == 0) P.tickets[bh] = 0;  // ready for the next launch on this stream
                     wrote_out = true;
+                }
+            }
+            if constexpr (kWeigh) {
+                if (wrote_out && sr.ok) {
+                    // the pair's maximum and sum, from this CTA's groups or from the splits' partials
+                    float MM = M, LL = 0.f;
+                    if (whole) {
+                        for (int gg = 0; gg < NG; ++gg) LL = fmaf(red[gg * RS + DH + 2], red[gg * RS + DH + 1], LL);
+                    } else {
+                        const int c_first = cut.first_cta_of(bh), count = cut.last_cta_of(bh) - c_first + 1;
+                        const float* pk = P.partials + (size_t)(c_first + bh) * (DH + 2);
+                        for (int k = 0; k < count; ++k) MM = fmaxf(MM, __ldcg(pk + (size_t)k * (DH + 2) + DH));
+                        for (int k = 0; k < count; ++k) {
+                            const float mk = __ldcg(pk + (size_t)k * (DH + 2) + DH);
+                            if (mk != -CUDART_INF_F) LL = fmaf(expo(mk - MM), __ldcg(pk + (size_t)k * (DH + 2) + DH + 1), LL);
+                        }
+                    }
+                    const float inv = 1.f / LL;   // the new token was scored: the sum is at least 1 at the maximum
+                    float* w = P.weights + (size_t)bh * P.Lmax;
+                    for (int r = sr.first + ctid; r < sr.row; r += nct) w[r] += expo(__ldcg(pair_scores + r) - MM) * inv;
+                    if (ctid == 0) {
+                        w[sr.row] = expo(__ldcg(pair_scores + sr.row) - MM) * inv;
+                        if (P.positions != nullptr) P.positions[(size_t)bh * P.Lmax + sr.row] = P.seen != nullptr ? P.seen[b] : sr.row;
+                    }
                 }
             }
             if (push && wrote_out) __threadfence_system();   // this thread's rows are at the peers before the pair is counted

@@ -17,6 +17,7 @@
 
 #include <memory>
 #include <string>
+#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -381,6 +382,75 @@ struct FastForwardAttn {
     }
     void tree_accept_per_sample(torch::Tensor path, torch::Tensor seq_lengths) { run_accept(target(), path, 0, &seq_lengths); }
 
+    // ---- a cache held at a budget of rows (ffa_attention_accumulate, ffa_evict) ----
+    void check_trackers(const torch::Tensor& weights, const torch::Tensor& positions) const
+    {
+        TORCH_CHECK(weights.is_cuda() && weights.device() == device && weights.scalar_type() == torch::kFloat && weights.is_contiguous() &&
+                        weights.dim() == 3 && weights.size(0) == B && weights.size(1) == H && weights.size(2) == Lmax,
+                    "FastForwardAttn: weights must be a contiguous float32 CUDA tensor [batch, heads, max_len]");
+        TORCH_CHECK(positions.is_cuda() && positions.device() == device && positions.scalar_type() == torch::kInt && positions.is_contiguous() &&
+                        positions.sizes() == weights.sizes(),
+                    "FastForwardAttn: positions must be a contiguous int32 CUDA tensor [batch, heads, max_len]");
+    }
+    torch::Tensor attention_accumulate(torch::Tensor q_, torch::Tensor k_, torch::Tensor v_, double softmax_scale, torch::Tensor seq_lengths,
+                                       torch::Tensor weights, torch::Tensor positions, torch::Tensor seen_, c10::optional<torch::Tensor> out_opt,
+                                       int64_t max_row)
+    {
+        const int64_t n = B * H * Dh;
+        auto prep = [&](const torch::Tensor& x, const char* name) {
+            TORCH_CHECK(x.is_cuda() && x.device() == device && dtype_code(x) == dtype && x.numel() == n, "FastForwardAttn: ", name,
+                        " must hold batch*heads*head_dim = ", n, " elements of the cache's dtype on the engine's device");
+            return x.contiguous();
+        };
+        torch::Tensor q = prep(q_, "q"), k = prep(k_, "k"), v = prep(v_, "v");
+        torch::Tensor rows = checked_rows(target(), seq_lengths, "seq_lengths"), seen = checked_rows(target(), seen_, "seen");
+        check_trackers(weights, positions);
+        TORCH_CHECK(max_row >= -1 && max_row < Lmax, "FastForwardAttn: max_row ", max_row, " outside [-1, ", Lmax, ")");
+        c10::cuda::CUDAGuard guard(device);
+        torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({B, H, Dh}, k_cache.options());
+        TORCH_CHECK(out.is_cuda() && out.device() == device && dtype_code(out) == dtype && out.is_contiguous() && out.numel() == n,
+                    "FastForwardAttn: out must be a contiguous tensor of batch*heads*head_dim elements on the engine's device");
+        if (!has_scores) bind_workspace(true);   // once, as for pruned steps
+        check(ffa_attention_accumulate(plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
+                                       (float)softmax_scale, (int)(max_row < 0 ? Lmax - 1 : max_row), rows.data_ptr<int>(),
+                                       weights.data_ptr<float>(), positions.data_ptr<int>(), seen.data_ptr<int>(),
+                                       at::cuda::getCurrentCUDAStream().stream()),
+              "accumulating attention");
+        return out;
+    }
+    torch::Tensor evict(torch::Tensor rows_, torch::Tensor weights, torch::Tensor positions, int64_t keep, int64_t recent, int64_t first,
+                        int64_t max_row)
+    {
+        torch::Tensor rows = checked_rows(target(), rows_, "seq_lengths");
+        check_trackers(weights, positions);
+        TORCH_CHECK(keep > 0 && keep <= Lmax, "FastForwardAttn: keep ", keep, " outside [1, ", Lmax, "]");
+        TORCH_CHECK(recent >= 0 && first >= 0 && recent <= keep && first <= keep - recent, "FastForwardAttn: need 0 <= recent (", recent,
+                    "), 0 <= first (", first, "), recent + first <= keep (", keep, ")");
+        TORCH_CHECK(max_row >= -1 && max_row <= Lmax, "FastForwardAttn: max_row ", max_row, " outside [-1, ", Lmax, "]");
+        c10::cuda::CUDAGuard guard(device);
+        torch::Tensor kept = torch::empty({B, H, keep}, torch::TensorOptions().dtype(torch::kInt).device(device));
+        check(ffa_evict(plan, k_cache.data_ptr(), v_cache.data_ptr(), weights.data_ptr<float>(), positions.data_ptr<int>(), rows.data_ptr<int>(),
+                        (int)(max_row < 0 ? Lmax : max_row), (int)keep, (int)recent, (int)first, kept.data_ptr<int>(),
+                        at::cuda::getCurrentCUDAStream().stream()),
+              "evict");
+        return kept;
+    }
+
+    // ---- beam search (ffa_cache_reorder) ----
+    void reorder(torch::Tensor parents_, int64_t rows, int64_t first_row)
+    {
+        TORCH_CHECK(parents_.is_cuda() && parents_.device() == device && parents_.scalar_type() == torch::kInt && parents_.dim() == 2 &&
+                        parents_.numel() == B,
+                    "FastForwardAttn: parents must be an int32 CUDA tensor [groups, beams] with groups * beams = batch = ", B);
+        TORCH_CHECK(first_row >= 0 && first_row <= rows && rows <= Lmax, "FastForwardAttn: need 0 <= first_row (", first_row, ") <= rows (", rows,
+                    ") <= ", Lmax);
+        torch::Tensor parents = parents_.contiguous();
+        c10::cuda::CUDAGuard guard(device);
+        check(ffa_cache_reorder(plan, k_cache.data_ptr(), v_cache.data_ptr(), parents.data_ptr<int>(), (int)parents.size(1), (int)first_row,
+                                (int)rows, at::cuda::getCurrentCUDAStream().stream()),
+              "reorder");
+    }
+
     std::pair<torch::Tensor, torch::Tensor> get_cache() { return std::make_pair(k_cache, v_cache); }
 
     void set_mode(const std::string& m)
@@ -662,12 +732,52 @@ struct PagedEngine {
     bool has_scores = false, want_mask = false;
 };
 
+// Selection over beams and vocabulary (ffa_beam_select): (scores fp32, parents int32, tokens int32), each [batch, num].
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> beam_select(torch::Tensor logits, torch::Tensor scores_, int64_t num,
+                                                                     c10::optional<torch::Tensor> finished_opt, int64_t pad_token)
+{
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 3 && logits.numel() > 0, "beam_select: logits must be a CUDA tensor [batch, beams, vocab]");
+    const int code = dtype_code(logits);
+    const int64_t B = logits.size(0), N = logits.size(1), V = logits.size(2);
+    TORCH_CHECK(N <= 32, "beam_select: ", N, " beams, at most 32");
+    TORCH_CHECK(num >= 1 && num <= 64, "beam_select: num ", num, " outside [1, 64]");
+    TORCH_CHECK(N * V < (int64_t(1) << 31) && B <= (int64_t(1) << 27), "beam_select: sizes exceed int range");
+    TORCH_CHECK(pad_token >= 0 && pad_token < V, "beam_select: pad_token ", pad_token, " outside [0, ", V, ")");
+    TORCH_CHECK(scores_.is_cuda() && scores_.device() == logits.device() && scores_.scalar_type() == torch::kFloat && scores_.dim() == 2 &&
+                    scores_.size(0) == B && scores_.size(1) == N,
+                "beam_select: scores must be a float32 CUDA tensor [batch, beams] on the logits' device");
+    // rows may lie apart (a padded vocabulary cut to its size), evenly and in order; anything else is copied
+    const bool even = (V == 1 || logits.stride(2) == 1) && (N == 1 || logits.stride(1) >= V) &&
+                      (B == 1 || N == 1 || logits.stride(0) == N * logits.stride(1)) && (B == 1 || N > 1 || logits.stride(0) >= V);
+    if (!even) logits = logits.contiguous();
+    const int64_t row_stride = N > 1 ? logits.stride(1) : B > 1 ? logits.stride(0) : V;
+    torch::Tensor scores = scores_.contiguous(), finished;
+    if (finished_opt.has_value()) {
+        TORCH_CHECK(finished_opt->is_cuda() && finished_opt->device() == logits.device() && finished_opt->scalar_type() == torch::kBool &&
+                        finished_opt->sizes() == scores.sizes(),
+                    "beam_select: finished must be a bool CUDA tensor [batch, beams] on the logits' device");
+        finished = finished_opt->contiguous();
+    }
+    c10::cuda::CUDAGuard guard(logits.device());
+    torch::Tensor best = torch::empty({B, num}, scores.options());
+    torch::Tensor parents = torch::empty({B, num}, scores.options().dtype(torch::kInt)), tokens = torch::empty_like(parents);
+    const int rc = ffa_beam_select(code, (int)B, (int)N, (int)V, row_stride, logits.data_ptr(), scores.data_ptr<float>(),
+                                   finished_opt.has_value() ? static_cast<const unsigned char*>(finished.data_ptr()) : nullptr, (int)pad_token,
+                                   (int)num, best.data_ptr<float>(), parents.data_ptr<int>(), tokens.data_ptr<int>(),
+                                   at::cuda::getCurrentCUDAStream().stream());
+    TORCH_CHECK(rc == FFA_OK, "beam_select: ", ffa_last_error());
+    return std::make_tuple(best, parents, tokens);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     m.doc() = "B200 decode masked multi-head attention behind the FastForwardAttention interface";
     m.def("launch_count", []() { return ffa_launch_count(); }, "kernels launched by the engine since load");
+    m.def("beam_select", &beam_select,
+          "the num best of scores[b, i] + log_softmax(logits[b, i])[v] over a sample's beams and vocabulary: (scores, parents, tokens)",
+          py::arg("logits"), py::arg("scores"), py::arg("num"), py::arg("finished") = py::none(), py::arg("pad_token") = 0);
     py::class_<FastForwardAttn>(m, "FastForwardAttn")
         .def(py::init<torch::Tensor, torch::Tensor, int64_t, bool>(), py::arg("K"), py::arg("V"), py::arg("max_timesteps"),
              py::arg("use_default_kernel_launch") = false)
@@ -704,6 +814,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
              "keep a verified path [B, A] (increasing tree indices, then -1): rows curr_timestep + path[b, i] -> curr_timestep + i",
              py::arg("path"), py::arg("curr_timestep"))
         .def("tree_accept_per_sample", &FastForwardAttn::tree_accept_per_sample, py::arg("path"), py::arg("seq_lengths"))
+        .def("attention_accumulate", &FastForwardAttn::attention_accumulate,
+             "decode step that adds each row's softmax weight to weights [B, H, max_len] (the new row's is set, and its position to seen[b])",
+             py::arg("q"), py::arg("k"), py::arg("v"), py::arg("softmax_scale"), py::arg("seq_lengths"), py::arg("weights"),
+             py::arg("positions"), py::arg("seen"), py::arg("out") = py::none(), py::arg("max_row") = -1)
+        .def("evict", &FastForwardAttn::evict,
+             "keep the `keep` heaviest of rows 0..seq_lengths[b]-1 (the `recent` newest and positions below `first` always); returns [B, H, keep], "
+             "the row that each row was before",
+             py::arg("seq_lengths"), py::arg("weights"), py::arg("positions"), py::arg("keep"), py::arg("recent") = 0, py::arg("first") = 0,
+             py::arg("max_row") = -1)
+        .def("reorder", &FastForwardAttn::reorder, "rows first_row..rows-1 of beam j <- beam parents[g, j], in place", py::arg("parents"),
+             py::arg("rows"), py::arg("first_row") = 0)
         .def("set_push_target", &FastForwardAttn::set_push_target, py::arg("gathered") = py::none(),
              "while set, exact steps push their output rows to the peers from the attention kernel (follow with peer_gather(phases=2))")
         .def("set_mode", &FastForwardAttn::set_mode, "'exact' (default) or 'round_like_torch'")

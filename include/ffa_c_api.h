@@ -199,6 +199,43 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
 int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* path, int path_len, int t, const int* seq_lengths,
                     const int* page_table, int max_pages, int page_rows, void* stream);
 
+/* ---- A cache held at a budget of rows: eviction by accumulated attention weight.  No counterpart in the reference.
+ * ffa_attention_accumulate is one exact decode step (ffa_attention with p = 0; always fp32 arithmetic, whatever the plan's mode)
+ * that also adds what each row was worth: with p[r] the softmax weights of the step,
+ *   weights[b, h, r] += p[r] for the cached rows, weights[b, h, row] = p[row] and positions[b, h, row] = seen[b] for the new one
+ * (row = t, or seq_lengths[b] as in ffa_attention with right padding; t is then their bound).  weights [batch, heads, max_len] fp32,
+ * positions [batch, heads, max_len] int32 or NULL, seen [batch] int32 or NULL (the row index).  The workspace must be sized with
+ * with_scores = 1.
+ * ffa_evict then keeps `keep` rows of every pair that has more: sample b uses rows 0..rows[b]-1, rows[b] <= max_rows <= 2^19.  Rows
+ * with a position below `first`, or among the `recent` newest positions (above the pair's largest position - recent), stay; of the others the heaviest
+ * stay, ties going to the lower row (NaN counts as the lightest; should more than `keep` rows be protected, the lowest of them stay).
+ * The survivors at rows >= keep move into the freed rows < keep, k-th to k-th in ascending order, K, V, weight and position;
+ * rows >= keep are left as they were, and the caller's rows[b] becomes min(rows[b], keep).
+ * kept [batch, heads, keep] receives the row that each row was before the call, -1 behind the sample's rows.  A sample whose
+ * rows[b] is out of range is left as it was (FFA_STATUS_BAD_LENGTH, kept -1).  recent + first <= keep. */
+int ffa_attention_accumulate(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache, void* out,
+                             float softmax_scale, int t, const int* seq_lengths, float* weights, int* positions, const int* seen,
+                             void* stream);
+int ffa_evict(ffa_plan_t* plan, void* k_cache, void* v_cache, float* weights, int* positions, const int* rows, int max_rows, int keep,
+              int recent, int first, int* kept, void* stream);
+
+/* ---- Beam search.  No counterpart in the reference (its kernel's cache indirection is disabled, attention.cu:1459-1491).
+ * ffa_beam_select: score(i, v) = scores[b, i] + logits[b, i, v] - logsumexp(logits[b, i, :]); the num best of every sample over its
+ * beams and vocabulary, best first, ties to the lowest i * vocab + v.  logits [batch, beams, vocab] of `dtype`, rows row_stride
+ * elements apart (aligned to their element type); scores fp32 [batch, beams]; finished NULL or one byte per beam: a finished beam offers only
+ * (its score unchanged, pad_token).  Only scores above -inf are candidates: a beam whose score is -inf or NaN, or whose logits
+ * hold NaN or +inf, has none, and what is missing is (-inf, parent 0, pad_token).  beams <= 32, num <= 64,
+ * beams * vocab < 2^31.  Needs no plan and no workspace.
+ * ffa_cache_reorder: rows [first_row, rows) of beam j <- beam parents[g, j] of its group, in place, in both caches and every
+ * head; the plan's batch is groups * beams, a group's beams adjacent; parents int32 (device).  Rows below first_row (a prompt
+ * that a group's beams share) and from `rows` on are left as they were, and so is a group with a parent outside [0, beams)
+ * (FFA_STATUS_BAD_INDEX). */
+int ffa_beam_select(int dtype, int batch, int beams, int vocab, long long row_stride, const void* logits, const float* scores,
+                    const unsigned char* finished, int pad_token, int num, float* out_scores, int* out_parents, int* out_tokens,
+                    void* stream);
+int ffa_cache_reorder(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* parents, int beams, int first_row, int rows,
+                      void* stream);
+
 /* The exact (p == 0, no per-sample lengths) decode step with NO caller-provided workspace and
  * no allocation of any kind inside the call.  It has no counterpart in the reference; it
  * exists for hosts that cannot allocate device memory when they call the engine: a server

@@ -73,3 +73,82 @@ def assert_within(got, want, bound, what=""):
     err = (got - want).abs()[fin]
     over = err > bound[fin]
     assert not over.any(), f"{what}: {int(over.sum())} of {over.numel()} off, worst {(err / bound[fin]).max().item():.2f} x the bound"
+
+
+def step_weights(q, k, v, k_cache, v_cache, scale, rows):
+    """One accumulating step: (out [B, H, D], its bound, p [B, H, L] with p[.., rows[b]] the new token's, p's bound), float64."""
+    B, H, L, D = k_cache.shape
+    one = torch.ones(1, 1, dtype=torch.bool, device=q.device)
+    out, bound = tree_attention(q.view(B, H, 1, D), k.view(B, H, 1, D), v.view(B, H, 1, D), k_cache, v_cache, one, scale, rows)
+    p = torch.zeros(B, H, L, dtype=torch.float64, device=q.device)
+    pb = torch.zeros_like(p)
+    for b in range(B):
+        n = int(rows[b])
+        for h in range(H):
+            keys = torch.cat([k_cache[b, h, :n], k.view(B, H, D)[b, h][None]]).double()
+            x = q.view(B, H, D)[b, h].double()
+            s = keys @ x * scale
+            w = torch.softmax(s, 0)
+            mag = ((keys.abs() @ x.abs()) * abs(scale)).max()
+            rel = 2 * ((D + 2) * U * mag + 4 * U * (1 + s.abs().max())) + (n + 8) * U
+            p[b, h, : n + 1], pb[b, h, : n + 1] = w, rel * w
+    return out[:, :, 0], bound[:, :, 0], p, pb
+
+
+def evict(caches, weights, positions, rows, keep, recent, first):
+    """Plain eviction of copies: (caches, weights, positions, kept)."""
+    caches = [c.clone() for c in caches]
+    weights, positions = weights.clone(), positions.clone()
+    B, H = weights.shape[:2]
+    kept = torch.full((B, H, keep), -1, dtype=torch.int32, device=weights.device)
+    for b in range(B):
+        n = int(rows[b])
+        for h in range(H):
+            src = list(range(min(n, keep)))
+            if n > keep:
+                w = weights[b, h, :n].tolist()
+                p = positions[b, h, :n].tolist()
+                newest = max(p)
+                safe = [x > newest - recent or x < first for x in p]
+                value = [-math.inf if x != x else x for x in w]
+                order = sorted(range(n), key=lambda r: (not safe[r], 0.0 if safe[r] else -value[r], 0 if safe[r] else w[r] != w[r], r))
+                stay = set(order[:keep])
+                freed = [r for r in range(keep) if r not in stay]
+                for d, s in zip(freed, sorted(r for r in stay if r >= keep)):
+                    src[d] = s
+                at = torch.tensor(src, device=weights.device)
+                for c in (*caches, weights, positions):
+                    c[b, h, :keep] = c[b, h][at].clone()
+            kept[b, h, : len(src)] = torch.tensor(src, dtype=torch.int32)
+    return caches, weights, positions, kept
+
+
+def beam_select(logits, scores, num, finished=None, pad_token=0):
+    """(scores float64, parents, tokens) by sorting every candidate."""
+    B, N, V = logits.shape
+    rows = []
+    for b in range(B):
+        cand = []
+        for i in range(N):
+            s0 = float(scores[b, i])
+            if finished is not None and bool(finished[b, i]):
+                cand.append((s0, i, pad_token))
+                continue
+            x = logits[b, i].double().cpu()
+            if torch.isnan(x).any() or (x == math.inf).any() or not (s0 > -math.inf):
+                continue
+            s = s0 + (x - torch.logsumexp(x, 0))
+            cand += [(float(s[t]), i, t) for t in torch.argsort(s, descending=True, stable=True)[:num].tolist()]
+        cand = sorted((c for c in cand if c[0] > -math.inf), key=lambda c: (-c[0], c[1], c[2]))
+        rows.append((cand + [(-math.inf, 0, pad_token)] * num)[:num])
+    t = torch.tensor(rows, dtype=torch.float64)
+    return t[..., 0], t[..., 1].int(), t[..., 2].int()
+
+
+def reorder(cache, parents, first_row, rows):
+    out = cache.clone()
+    N = parents.shape[1]
+    for g, ps in enumerate(parents.tolist()):
+        for j, p in enumerate(ps):
+            out[g * N + j, :, first_row:rows] = cache[g * N + p, :, first_row:rows]
+    return out

@@ -54,3 +54,49 @@ def test_tree_scratch(plan):
     assert L.ffa_tree_scratch_bytes(p, 1, 8, 10, None) == ARG
     assert L.ffa_tree_scratch_bytes(p, 1, 2000, 10, C.byref(n)) == RANGE
     assert L.ffa_tree_scratch_bytes(None, 1, 8, 10, C.byref(n)) == ARG
+
+
+@pytest.mark.parametrize("kw,code", [(dict(plan=None), ARG), (dict(kc=ODD), ARG), (dict(w=None), ARG), (dict(pos=None), ARG), (dict(rows=None), ARG), (dict(kept=None), ARG),
+                                     (dict(most=-1), RANGE), (dict(most=4097), RANGE), (dict(keep=0), RANGE), (dict(keep=4097), RANGE), (dict(recent=-1), RANGE),
+                                     (dict(recent=90, first=11), RANGE), (dict(recent=2 ** 31 - 1, first=2 ** 31 - 1), RANGE), (dict(), ARG)])
+def test_evict_refusals(plan, kw, code):
+    L, p = plan
+    a = dict(plan=p, kc=P16, vc=P16, w=P16, pos=P16, rows=P16, most=4096, keep=100, recent=10, first=4, kept=P16, stream=None)
+    a.update(kw)
+    assert L.ffa_evict(*a.values()) == code, L.ffa_last_error()
+
+
+def test_evict_refuses_more_rows_than_a_selection_holds():
+    L = capi.lib()
+    p = C.c_void_p()
+    capi.check(L.ffa_plan_create_offline(capi.F16, 1, 1, 64, 1 << 20, 0, SMS, SMEM_CTA, SMEM_SM, C.byref(p)))
+    assert L.ffa_evict(p, P16, P16, P16, P16, P16, (1 << 19) + 1, 100, 0, 0, P16, None) == RANGE
+    L.ffa_plan_destroy(p)
+
+
+def test_accumulate_refusals(plan):
+    L, p = plan
+    assert L.ffa_attention_accumulate(None, P16, P16, P16, P16, P16, P16, 1.0, 5, None, P16, None, None, None) == ARG
+    assert L.ffa_attention_accumulate(p, P16, P16, P16, P16, P16, P16, 1.0, 5, None, None, None, None, None) == ARG
+    assert L.ffa_attention_accumulate(p, P16, P16, P16, P16, P16, P16, 1.0, 5, None, P16, None, None, None) == ARG   # offline
+
+
+@pytest.mark.parametrize("kw,code", [(dict(dtype=3), -1), (dict(batch=0), RANGE), (dict(vocab=0), RANGE), (dict(beams=0), RANGE), (dict(beams=33), RANGE), (dict(num=0), RANGE),
+                                     (dict(num=65), RANGE), (dict(stride=99), RANGE), (dict(pad=-1), RANGE), (dict(pad=100), RANGE), (dict(logits=None), ARG),
+                                     (dict(logits=C.c_void_p(4097)), ARG), (dict(scores=None), ARG), (dict(tokens=None), ARG),
+                                     (dict(beams=32, vocab=1 << 27, stride=1 << 27), RANGE)])
+def test_beam_select_refusals(kw, code):
+    a = dict(dtype=capi.F16, batch=2, beams=4, vocab=100, stride=100, logits=P16, scores=P16, finished=None, pad=0, num=8, best=P16, parents=P16,
+             tokens=P16, stream=None)
+    a.update(kw)
+    L = capi.lib()
+    assert L.ffa_beam_select(*a.values()) == code, L.ffa_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [(dict(plan=None), ARG), (dict(kc=None), ARG), (dict(vc=ODD), ARG), (dict(parents=None), ARG), (dict(beams=0), RANGE), (dict(beams=3), RANGE),
+                                     (dict(beams=64), RANGE), (dict(first=-1), RANGE), (dict(first=51), RANGE), (dict(rows=4097), RANGE), (dict(), ARG)])
+def test_reorder_refusals(plan, kw, code):
+    L, p = plan
+    a = dict(plan=p, kc=P16, vc=P16, parents=P16, beams=4, first=0, rows=50, stream=None)
+    a.update(kw)
+    assert L.ffa_cache_reorder(*a.values()) == code, L.ffa_last_error()
