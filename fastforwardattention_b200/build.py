@@ -29,7 +29,7 @@ COMMON_HEADERS = ["ffa_internal.h", "ffa_device_common.cuh", "ffa_launch.cuh"]
 # every source with the headers it includes: what makes its object stale
 CUDA_SOURCES = {
     "ffa_decode_kernels.cu": [*COMMON_HEADERS, "ffa_stream_kernel.cuh", "ffa_prune_kernels.cuh", "ffa_prune_stream_kernel.cuh"],
-    "ffa_tree_kernels.cu": [*COMMON_HEADERS, "ffa_tree_kernel.cuh"],
+    "ffa_tree_kernels.cu": [*COMMON_HEADERS, "ffa_tree_kernel.cuh", "ffa_tree_umma_kernel.cuh"],
     "ffa_evict_kernels.cu": COMMON_HEADERS,
     "ffa_beam_kernels.cu": COMMON_HEADERS,
     "ffa_strategies_api.cu": ["ffa_internal.h", "ffa_plan.h", API_HEADER],

@@ -111,12 +111,15 @@ struct FfaTreeParams {
     int B, H, Lmax, t, groups, tokens;
     float scale;
     int splits, row_tiles;       // CTAs per (pair, tile of query rows); tiles of query rows per pair
-    float* partials;             // [B*H][row_tiles][splits][tile rows][Dh + 2]; null when splits == 1
+    int part_rows;               // query rows of a partial result: a tile's, or all there are
+    float* partials;             // [B*H][row_tiles][splits][part_rows][Dh + 4]; null when splits == 1
     int* tickets;                // [B*H][kTreeTicketsPerPair], zero between launches
     int* status;
     const int* page_table;       // as in FfaStepParams
     int max_pages, page_rows;
 };
+// Floats of a partial result's row: the weighted sum, its maximum, its sum of exponentials, and two to keep rows 16-byte aligned
+constexpr int ffa_tree_part_stride(int head_dim) { return head_dim + 4; }
 // Moving the accepted path of a tree to the front of its rows (ffa_tree_accept).
 struct FfaAcceptParams {
     void* k_cache;
@@ -128,8 +131,8 @@ struct FfaAcceptParams {
     const int* page_table;
     int max_pages, page_rows;
 };
-int ffa_k_tree_rows(int dtype, int rows);      // query rows per CTA
-int ffa_k_tree_smem(int dtype, int head_dim, int rows);
+// query rows per CTA, key rows per tile and resident CTAs per SM of the kernel that takes this type and number of query rows
+void ffa_k_tree_shape(int dtype, int head_dim, int rows, int* tile_rows, int* tile_keys, int* ctas_per_sm);
 int ffa_k_tree_prepare(int dtype, int head_dim);
 int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaStream_t stream);
 int ffa_k_tree_accept(const FfaAcceptParams& P, cudaStream_t stream);

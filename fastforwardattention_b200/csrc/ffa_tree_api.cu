@@ -11,28 +11,40 @@ namespace {
 
 // The cut of a tree attention: tiles of query rows per pair, and CTAs per (pair, tile of query rows).
 struct TreeShape {
-    int tile_rows, row_tiles, splits;
+    int tile_rows, row_tiles, part_rows, splits;
 };
 
+// A CTA's time is its key tiles plus a fixed part (start, first tile, epilogue: a few tiles' worth), and more for the merge when a
+// pair is split.  All CTAs of a full wave share HBM; a CTA that is nearly alone still takes a tile every third of a microsecond.  The
+// number of splits is the one with the smallest sum over the waves.
 TreeShape tree_shape(const ffa_plan* p, int groups, int tokens, int t)
 {
     TreeShape s;
     const int rows = groups * tokens;
-    s.tile_rows = ffa_k_tree_rows(p->dtype, rows);
+    int tile_keys, cps;
+    ffa_k_tree_shape(p->dtype, p->Dh, rows, &s.tile_rows, &tile_keys, &cps);
     s.row_tiles = (rows + s.tile_rows - 1) / s.tile_rows;
-    // two CTAs per SM; a split has at least four key tiles
-    const long long items = (long long)p->B * p->H * s.row_tiles;
-    const long long tiles = (t + 31) / 32 + (tokens + 31) / 32;
-    long long splits = 2LL * p->sms / items;
-    if (splits > tiles / 4) splits = tiles / 4;
-    s.splits = (int)(splits < 1 ? 1 : splits);
+    s.part_rows = rows < s.tile_rows ? rows : s.tile_rows;
+    const long long items = (long long)p->B * p->H * s.row_tiles, slots = (long long)p->sms * cps;
+    const long long tiles = (t + tile_keys - 1) / tile_keys + (tokens + tile_keys - 1) / tile_keys;
+    const double tile_us = 2.0 * tile_keys * p->Dh * ffa_elem_size(p->dtype) / 6.6e6;   // of the whole device's HBM bandwidth
+    double best = 0;
+    s.splits = 1;
+    for (long long splits = 1; splits <= tiles && splits <= 64; ++splits) {
+        const long long ctas = items * splits, full = ctas / slots, rest = ctas % slots;
+        const double run = (double)((tiles + splits - 1) / splits);
+        const double fixed = 3.0 + (splits > 1 ? 1.5 + 0.1 * splits : 0.0);
+        auto wave = [&](long long n) { return n == 0 ? 0.0 : run * (n * tile_us > 0.35 ? n * tile_us : 0.35) + fixed; };
+        const double us = full * wave(slots) + wave(rest);
+        if (splits == 1 || us < best) best = us, s.splits = (int)splits;
+    }
     return s;
 }
 
 size_t tree_partials_bytes(const ffa_plan* p, const TreeShape& s)
 {
     if (s.splits <= 1) return 0;
-    return (size_t)p->B * p->H * s.row_tiles * s.splits * s.tile_rows * (p->Dh + 2) * sizeof(float);
+    return (size_t)p->B * p->H * s.row_tiles * s.splits * s.part_rows * ffa_tree_part_stride(p->Dh) * sizeof(float);
 }
 
 int check_sizes(const ffa_plan* plan, int groups, int tokens, int t)
@@ -100,7 +112,7 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
     P.seq_lengths = seq_lengths, P.right_or_no_padding = right_or_no_padding != 0;
     P.B = plan->B, P.H = plan->H, P.Lmax = plan->Lmax, P.t = t, P.groups = groups, P.tokens = tokens;
     P.scale = softmax_scale;
-    P.splits = s.splits, P.row_tiles = s.row_tiles;
+    P.splits = s.splits, P.row_tiles = s.row_tiles, P.part_rows = s.part_rows;
     P.partials = static_cast<float*>(scratch), P.tickets = plan->tree_tickets, P.status = plan->status;
     P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows;
     r = ffa_k_tree_attention(plan->dtype, plan->Dh, P, static_cast<cudaStream_t>(stream));

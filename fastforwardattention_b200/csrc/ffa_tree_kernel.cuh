@@ -55,22 +55,22 @@ __device__ __forceinline__ void tree_append(const FfaTreeParams& P, int bh, int 
     }
 }
 
-// Combines the splits' partials of one tile of query rows in split order: [splits][tile_rows][DH + 2] floats, a row being the
-// weighted sum, its maximum and its sum of exponentials.
+// Combines the splits' partials of one tile of query rows in split order ([splits][part_rows][stride] floats).
 template <typename T, int DH, bool kLog2>
-__device__ __forceinline__ void tree_merge(const float* part, int splits, int tile_rows, int rows, T* out, int tid, int threads)
+__device__ __forceinline__ void tree_merge(const float* part, int splits, int part_rows, int rows, T* out, int tid, int threads)
 {
     for (int i = tid; i < rows * DH; i += threads) {
         const int r = i / DH, d = i - r * DH;
-        const float* pr = part + (size_t)r * (DH + 2);
-        const size_t step = (size_t)tile_rows * (DH + 2);
+        const float* pr = part + (size_t)r * ffa_tree_part_stride(DH);
+        const size_t step = (size_t)part_rows * ffa_tree_part_stride(DH);
         float M = -CUDART_INF_F;
         for (int s = 0; s < splits; ++s) M = fmaxf(M, __ldcg(pr + s * step + DH));
         float A = 0.f, L = 0.f;
         for (int s = 0; s < splits; ++s) {
             const float ms = __ldcg(pr + s * step + DH);
             const float w = ms == -CUDART_INF_F ? 0.f : (kLog2 ? fast_exp2(ms - M) : expf(ms - M));
-            A = fmaf(w, __ldcg(pr + s * step + d), A);
+            const float a = __ldcg(pr + s * step + d);
+            A = isfinite(a) ? fmaf(w, a, A) : A + a;   // a split's infinity stays one however small its share is
             L = fmaf(w, __ldcg(pr + s * step + DH + 1), L);
         }
         Elem<T>::store(out + i, L > 0.f ? A / L : 0.f);
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
 
     const bool whole = cut.splits == 1;
     const size_t tile_index = (size_t)cut.bh * P.row_tiles + cut.rt;
-    float* part = whole ? nullptr : P.partials + (tile_index * P.splits + cut.split) * BM * (DH + 2);
+    float* part = whole ? nullptr : P.partials + (tile_index * P.splits + cut.split) * P.part_rows * ffa_tree_part_stride(DH);
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
         const int r = warp * RPW + i;
@@ -229,9 +229,9 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
             const int d = lane + 32 * x;
             if (DH % 32 != 0 && d >= DH) break;
             if (whole) Elem<T>::store(out + r * DH + d, L > 0.f ? acc[i][x] / L : 0.f);
-            else part[r * (DH + 2) + d] = acc[i][x];
+            else part[r * ffa_tree_part_stride(DH) + d] = acc[i][x];
         }
-        if (!whole && lane == 0) part[r * (DH + 2) + DH] = m[i], part[r * (DH + 2) + DH + 1] = L;
+        if (!whole && lane == 0) part[r * ffa_tree_part_stride(DH) + DH] = m[i], part[r * ffa_tree_part_stride(DH) + DH + 1] = L;
     }
     if (whole) return;
     // whoever arrives last merges; nobody waits (the fences are those of the decode kernels' merge)
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
     }
     __syncthreads();
     if (last) {
-        tree_merge<T, DH, false>(P.partials + tile_index * P.splits * BM * (DH + 2), cut.splits, BM, rows, out, tid, kTreeThreads);
+        tree_merge<T, DH, false>(P.partials + tile_index * P.splits * P.part_rows * ffa_tree_part_stride(DH), cut.splits, P.part_rows, rows, out, tid, kTreeThreads);
         if (tid == 0) *ticket = 0;
     }
 }

@@ -1,5 +1,7 @@
-// Launch glue of the tree attention kernels (ffa_tree_kernel.cuh).
+// Launch glue of the tree attention: fp16 and bf16 on the tensor cores (ffa_tree_umma_kernel.cuh), fp32 on the CUDA cores
+// (ffa_tree_kernel.cuh; the tensor cores have no product of fp32's precision), and the acceptance of a path.
 #include "ffa_tree_kernel.cuh"
+#include "ffa_tree_umma_kernel.cuh"
 
 #include "ffa_internal.h"
 #include "ffa_launch.cuh"
@@ -8,56 +10,118 @@ using namespace ffa_dev;
 
 namespace {
 
-// query rows per warp: a pair with at most 8 rows takes one per warp (eight times the CTA's warps share the tile's keys among
-// fewer rows otherwise)
+// query rows per warp of the CUDA-core kernel: a pair with at most 8 rows takes one per warp (with four, a quarter of the warps would
+// have them all)
 constexpr int kManyRows = 4;
 
-template <typename T, int DH, typename F>
+template <int DH, typename F>
 int with_rows(int rows, F&& f)
 {
-    return rows <= kTreeWarps ? f(ffa_tree_simt_kernel<T, DH, 1>) : f(ffa_tree_simt_kernel<T, DH, kManyRows>);
+    return rows <= kTreeWarps ? f(ffa_tree_simt_kernel<float, DH, 1>) : f(ffa_tree_simt_kernel<float, DH, kManyRows>);
+}
+
+int simt_rows(int rows) { return rows <= kTreeWarps ? kTreeWarps : kTreeWarps * kManyRows; }
+int simt_smem(int head_dim, int rows) { return simt_rows(rows) * head_dim * 4 + 4 * kTreeKeys * (head_dim * 4 + 16); }
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// the driver's encoder, looked up once (nothing here links against the driver library)
+EncodeTiled encoder()
+{
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// rows of head_dim 16-bit elements, in boxes of 64 columns (128 swizzled bytes) and box_rows rows; columns behind head_dim and rows
+// behind `rows` read as zeros
+int encode(CUtensorMap* map, int dtype, const void* base, int head_dim, long long rows, int box_rows)
+{
+    const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)head_dim * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, steps[2] = {1, 1};
+    const CUresult r = encoder()(map, dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base),
+                                 dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+template <typename F>
+int dispatch16(int dtype, int head_dim, F&& f)
+{
+    return dispatch(dtype, head_dim, [&](auto t, auto dh) -> int {
+        if constexpr (sizeof(decltype(t)) == 2) return f(t, dh);
+        else return (int)cudaErrorInvalidValue;
+    });
+}
+template <typename F>
+int dispatch32(int head_dim, F&& f)
+{
+    return dispatch(0, head_dim, [&](auto t, auto dh) -> int {
+        if constexpr (sizeof(decltype(t)) == 4) return f(dh);
+        else return (int)cudaErrorInvalidValue;
+    });
 }
 
 }  // namespace
 
-int ffa_k_tree_rows(int dtype, int rows)
+void ffa_k_tree_shape(int dtype, int head_dim, int rows, int* tile_rows, int* tile_keys, int* ctas_per_sm)
 {
-    (void)dtype;
-    return rows <= kTreeWarps ? kTreeWarps : kTreeWarps * kManyRows;
-}
-
-int ffa_k_tree_smem(int dtype, int head_dim, int rows)
-{
-    const int rowb = head_dim * (dtype == 0 ? 4 : 2);
-    return ffa_k_tree_rows(dtype, rows) * head_dim * 4 + 4 * kTreeKeys * (rowb + 16);
+    if (dtype == 0) *tile_rows = simt_rows(rows), *tile_keys = kTreeKeys, *ctas_per_sm = 2;
+    else *tile_rows = kUmmaRows, *tile_keys = kUmmaKeys, *ctas_per_sm = umma_ctas_per_sm(head_dim);
 }
 
 int ffa_k_tree_prepare(int dtype, int head_dim)
 {
-    return dispatch(dtype, head_dim, [&](auto t, auto dh) -> int {
+    if (dtype == 0)
+        return dispatch32(head_dim, [&](auto dh) -> int {
+            constexpr int DH = decltype(dh)::value;
+            for (int rows : {1, kTreeMaxRows}) {
+                const int e = with_rows<DH>(rows, [&](auto kernel) {
+                    return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, simt_smem(DH, rows));
+                });
+                if (e != 0) return e;
+            }
+            return 0;
+        });
+    if (encoder() == nullptr) return (int)cudaErrorNotSupported;
+    return dispatch16(dtype, head_dim, [&](auto t, auto dh) -> int {
         using T = decltype(t);
         constexpr int DH = decltype(dh)::value;
-        for (int rows : {1, kTreeMaxRows}) {
-            const int e = with_rows<T, DH>(rows, [&](auto kernel) {
-                return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 ffa_k_tree_smem(dtype, DH, rows));
-            });
-            if (e != 0) return e;
-        }
-        return 0;
+        return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(ffa_tree_umma_kernel<T, DH>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         umma_smem(DH));
     });
 }
 
 int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaStream_t stream)
 {
-    return dispatch(dtype, head_dim, [&](auto t, auto dh) -> int {
+    const int rows = P.groups * P.tokens;
+    const int grid = P.B * P.H * P.row_tiles * P.splits;
+    if (dtype == 0)
+        return dispatch32(head_dim, [&](auto dh) -> int {
+            constexpr int DH = decltype(dh)::value;
+            return with_rows<DH>(rows, [&](auto kernel) { return (int)launch_pdl(kernel, grid, kTreeThreads, simt_smem(DH, rows), 0, true, stream, P); });
+        });
+    FfaTreeUmmaParams U;
+    U.p = P;
+    const long long pairs = (long long)P.B * P.H;
+    // a pool's number of pages is not known here: its bound is only there to be larger than every row
+    const long long cache_rows = P.page_table != nullptr ? 0x7fffffffLL : pairs * P.Lmax;
+    int e = encode(&U.q, dtype, P.q, head_dim, pairs * rows, kQBoxRows);
+    if (e == 0) e = encode(&U.k_new, dtype, P.k, head_dim, pairs * P.tokens, kUmmaKeys);
+    if (e == 0) e = encode(&U.v_new, dtype, P.v, head_dim, pairs * P.tokens, kUmmaKeys);
+    if (e == 0) e = encode(&U.k_cache, dtype, P.k_cache, head_dim, cache_rows, kUmmaKeys);
+    if (e == 0) e = encode(&U.v_cache, dtype, P.v_cache, head_dim, cache_rows, kUmmaKeys);
+    if (e != 0) return e;
+    return dispatch16(dtype, head_dim, [&](auto t, auto dh) -> int {
         using T = decltype(t);
         constexpr int DH = decltype(dh)::value;
-        const int rows = P.groups * P.tokens;
-        const int grid = P.B * P.H * P.row_tiles * P.splits;
-        return with_rows<T, DH>(rows, [&](auto kernel) {
-            return (int)launch_pdl(kernel, grid, kTreeThreads, ffa_k_tree_smem(dtype, DH, rows), 0, true, stream, P);
-        });
+        return (int)launch_pdl(ffa_tree_umma_kernel<T, DH>, grid, kUmmaThreads, umma_smem(DH), 0, true, stream, U);
     });
 }
 
