@@ -60,7 +60,7 @@ constexpr long long kAlignedBelowUnitsPerSlot = 200;
 constexpr double kStreamPruneAboveBytes = 1e9;
 
 struct Carve {
-    size_t status, tickets, tree_tickets, partials, scores, total;
+    size_t status, tickets, partials, scores, total;
 };
 Carve carve(const ffa_plan* p, bool with_scores)
 {
@@ -69,7 +69,6 @@ Carve carve(const ffa_plan* p, bool with_scores)
     size_t off = 0;
     c.status = off, off += 256;
     c.tickets = off, off += align_up(BH * sizeof(int), 256);
-    c.tree_tickets = off, off += align_up(BH * kTreeTicketsPerPair * sizeof(int), 256);
     c.partials = off, off += align_up(((size_t)p->max_grid + BH) * (p->Dh + 2) * sizeof(float), 256);
     c.scores = off;
     if (with_scores) off += align_up(BH * (size_t)score_stride(p->Lmax) * sizeof(float), 256);
@@ -552,7 +551,6 @@ int ffa_workspace_bind(ffa_plan_t* plan, void* workspace, size_t bytes, void* st
     plan->ws = workspace, plan->ws_bytes = bytes;
     plan->status = reinterpret_cast<int*>(base + small.status);
     plan->tickets = reinterpret_cast<int*>(base + small.tickets);
-    plan->tree_tickets = reinterpret_cast<int*>(base + small.tree_tickets);
     plan->partials = reinterpret_cast<float*>(base + small.partials);
     plan->scores = bytes >= big.total ? reinterpret_cast<float*>(base + big.scores) : nullptr;
     return FFA_OK;

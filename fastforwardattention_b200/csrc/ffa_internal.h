@@ -90,10 +90,8 @@ int ffa_k_wait_selftest(int* status, unsigned long long limit_ns, unsigned long 
 // all-gather of the step outputs: a few CTAs per rank
 int ffa_k_peer_gather(FfaPeerGatherParams G, cudaStream_t stream);
 
-// Arrival counters per pair: one per tile of query rows of a tree attention (at most 1024 rows, tiles of 32 or more; 8 rows only
-// where a pair has no more than 8).
-constexpr int kTreeTicketsPerPair = 32;
-constexpr int kTreeMaxRows = 1024;   // groups * tokens
+constexpr int kTreeMaxRows = 1024;   // groups * tokens of a tree attention
+constexpr int kTreeMaxSplits = 64;   // CTAs that share a pair's key tiles
 
 // One attention step for a tree of drafted tokens (ffa_tree_attention).  Rows r = g * tokens + t of a pair are query head
 // h * groups + g at drafted token t.
@@ -111,9 +109,9 @@ struct FfaTreeParams {
     int B, H, Lmax, t, groups, tokens;
     float scale;
     int splits, row_tiles;       // CTAs per (pair, tile of query rows); tiles of query rows per pair
+    int tile_rows;
     int part_rows;               // query rows of a partial result: a tile's, or all there are
     float* partials;             // [B*H][row_tiles][splits][part_rows][Dh + 4]; null when splits == 1
-    int* tickets;                // [B*H][kTreeTicketsPerPair], zero between launches
     int* status;
     const int* page_table;       // as in FfaStepParams
     int max_pages, page_rows;

@@ -22,7 +22,6 @@ struct ffa_plan {
     size_t ws_bytes;
     int* status;
     int* tickets;
-    int* tree_tickets;   // [B*H][kTreeTicketsPerPair]: arrival counters of the tree attention's splits
     float* partials;
     float* scores;
     int max_grid;

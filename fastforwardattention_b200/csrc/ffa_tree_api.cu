@@ -30,7 +30,7 @@ TreeShape tree_shape(const ffa_plan* p, int groups, int tokens, int t)
     const double tile_us = 2.0 * tile_keys * p->Dh * ffa_elem_size(p->dtype) / 6.6e6;   // of the whole device's HBM bandwidth
     double best = 0;
     s.splits = 1;
-    for (long long splits = 1; splits <= tiles && splits <= 64; ++splits) {
+    for (long long splits = 1; splits <= tiles && splits <= kTreeMaxSplits; ++splits) {
         const long long ctas = items * splits, full = ctas / slots, rest = ctas % slots;
         const double run = (double)((tiles + splits - 1) / splits);
         const double fixed = 3.0 + (splits > 1 ? 1.5 + 0.1 * splits : 0.0);
@@ -112,12 +112,12 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
     P.seq_lengths = seq_lengths, P.right_or_no_padding = right_or_no_padding != 0;
     P.B = plan->B, P.H = plan->H, P.Lmax = plan->Lmax, P.t = t, P.groups = groups, P.tokens = tokens;
     P.scale = softmax_scale;
-    P.splits = s.splits, P.row_tiles = s.row_tiles, P.part_rows = s.part_rows;
-    P.partials = static_cast<float*>(scratch), P.tickets = plan->tree_tickets, P.status = plan->status;
+    P.splits = s.splits, P.row_tiles = s.row_tiles, P.part_rows = s.part_rows, P.tile_rows = s.tile_rows;
+    P.partials = static_cast<float*>(scratch), P.status = plan->status;
     P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows;
     r = ffa_k_tree_attention(plan->dtype, plan->Dh, P, static_cast<cudaStream_t>(stream));
     if (r != 0) return ffa_cuda_fail(r, "tree attention launch");
-    ffa_count_launches(1);
+    ffa_count_launches(s.splits > 1 ? 2 : 1);
     return FFA_OK;
 }
 

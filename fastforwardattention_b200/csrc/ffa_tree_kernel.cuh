@@ -55,25 +55,81 @@ __device__ __forceinline__ void tree_append(const FfaTreeParams& P, int bh, int 
     }
 }
 
-// Combines the splits' partials of one tile of query rows in split order ([splits][part_rows][stride] floats).
-template <typename T, int DH, bool kLog2>
-__device__ __forceinline__ void tree_merge(const float* part, int splits, int part_rows, int rows, T* out, int tid, int threads)
+// A split that has no key tiles (a sample shorter than the bound, or refused) leaves an empty partial result: the merge reads
+// nothing else of it.
+__device__ __forceinline__ float* tree_partial(const FfaTreeParams& P, int bh, int rt, int split, int dh)
 {
-    for (int i = tid; i < rows * DH; i += threads) {
-        const int r = i / DH, d = i - r * DH;
-        const float* pr = part + (size_t)r * ffa_tree_part_stride(DH);
-        const size_t step = (size_t)part_rows * ffa_tree_part_stride(DH);
-        float M = -CUDART_INF_F;
-        for (int s = 0; s < splits; ++s) M = fmaxf(M, __ldcg(pr + s * step + DH));
-        float A = 0.f, L = 0.f;
-        for (int s = 0; s < splits; ++s) {
-            const float ms = __ldcg(pr + s * step + DH);
-            const float w = ms == -CUDART_INF_F ? 0.f : (kLog2 ? fast_exp2(ms - M) : expf(ms - M));
-            const float a = __ldcg(pr + s * step + d);
-            A = isfinite(a) ? fmaf(w, a, A) : A + a;   // a split's infinity stays one however small its share is
-            L = fmaf(w, __ldcg(pr + s * step + DH + 1), L);
+    return P.partials + (((size_t)bh * P.row_tiles + rt) * P.splits + split) * P.part_rows * ffa_tree_part_stride(dh);
+}
+__device__ __forceinline__ void tree_empty_partial(float* part, int rows, int dh, int tid, int threads)
+{
+    for (int r = tid; r < rows; r += threads) {
+        part[(size_t)r * ffa_tree_part_stride(dh) + dh] = -CUDART_INF_F;
+        part[(size_t)r * ffa_tree_part_stride(dh) + dh + 1] = 0.f;
+    }
+}
+
+// Combines the splits' partial results in split order.  A warp per query row: the lanes find the row's maximum and sum (a split
+// each), then take the columns (16 bytes of every partial at a time, eight partials in flight).  A kernel of its own rather than
+// the work of the CTA that arrives last: 128 rows of nine splits are 600 KB, which one CTA takes 20 us and more to read and the
+// whole device a few; launched with programmatic overlap it costs about what the arrival counter and its fences did.
+constexpr int kMergeWarps = 4;
+template <typename T, int DH, bool kLog2>
+__global__ void __launch_bounds__(32 * kMergeWarps) ffa_tree_merge_kernel(const FfaTreeParams P)
+{
+    constexpr int STRIDE = ffa_tree_part_stride(DH), VECS = DH / 4, VPL = (VECS + 31) / 32;
+    __shared__ float weight[kMergeWarps][kTreeMaxSplits];
+    pdl_release();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int R = P.groups * P.tokens;
+    const long long row = (long long)blockIdx.x * kMergeWarps + warp;
+    if (row >= (long long)P.B * P.H * R) return;
+    const int bh = (int)(row / R), r = (int)(row - (long long)bh * R), rt = r / P.tile_rows;
+    const float* part = tree_partial(P, bh, rt, 0, DH) + (size_t)(r - rt * P.tile_rows) * STRIDE;
+    const size_t step = (size_t)P.part_rows * STRIDE;
+    auto expo = [](float x) { return kLog2 ? fast_exp2(x) : expf(x); };
+    float M = -CUDART_INF_F;
+    for (int s = lane; s < P.splits; s += 32) M = fmaxf(M, part[s * step + DH]);
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float L = 0.f;
+    for (int s = lane; s < P.splits; s += 32) {
+        const float m = part[s * step + DH];
+        const float w = m == -CUDART_INF_F ? 0.f : expo(m - M);
+        // an empty split has no maximum: its columns are not read (a weight of -1); one whose weight vanished still is
+        weight[warp][s] = m == -CUDART_INF_F ? -1.f : w;
+        L = fmaf(w, part[s * step + DH + 1], L);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+    __syncwarp();
+    T* out = static_cast<T*>(P.out) + (size_t)row * DH;
+#pragma unroll
+    for (int x = 0; x < VPL; ++x) {
+        const int c = lane + 32 * x;
+        if (c >= VECS) break;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < P.splits; s0 += 8) {
+            float4 a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (s0 + i < P.splits && weight[warp][s0 + i] >= 0.f) a[i] = *reinterpret_cast<const float4*>(part + (s0 + i) * step + 4 * c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (s0 + i >= P.splits) continue;
+                const float w = weight[warp][s0 + i];
+                if (!(w >= 0.f)) continue;   // empty, or NaN: then the sum is NaN too
+                // a split's infinity stays one however small its share is
+                acc.x = isfinite(a[i].x) ? fmaf(w, a[i].x, acc.x) : acc.x + a[i].x;
+                acc.y = isfinite(a[i].y) ? fmaf(w, a[i].y, acc.y) : acc.y + a[i].y;
+                acc.z = isfinite(a[i].z) ? fmaf(w, a[i].z, acc.z) : acc.z + a[i].z;
+                acc.w = isfinite(a[i].w) ? fmaf(w, a[i].w, acc.w) : acc.w + a[i].w;
+            }
         }
-        Elem<T>::store(out + i, L > 0.f ? A / L : 0.f);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        Elem<T>::store(out + 4 * c, acc.x * inv), Elem<T>::store(out + 4 * c + 1, acc.y * inv);
+        Elem<T>::store(out + 4 * c + 2, acc.z * inv), Elem<T>::store(out + 4 * c + 3, acc.w * inv);
     }
 }
 
@@ -89,20 +145,19 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
     extern __shared__ __align__(128) unsigned char smem[];
     float* qs = reinterpret_cast<float*>(smem);                       // [BM][DH], scaled
     unsigned char* ring = smem + (size_t)BM * DH * 4;                  // [2 stages][K | V][BN][PITCH]
-    __shared__ int last;
 
     pdl_release();
     pdl_wait();
     const TreeCut<BN> cut(P);
-    if (cut.split >= cut.splits) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int R = P.groups * P.tokens, row0 = cut.rt * BM, rows = min(BM, R - row0);
+    const bool whole = P.splits == 1;
     T* out = static_cast<T*>(P.out) + ((size_t)cut.bh * R + row0) * DH;
-    if (!cut.sr.ok) {   // refused: zeros, nothing appended
-        if (cut.split == 0) {
-            for (int i = tid; i < rows * DH; i += kTreeThreads) Elem<T>::store(out + i, 0.f);
-            if (tid == 0) atomicOr(P.status, kStatusBadLength);
-        }
+    float* part = whole ? nullptr : tree_partial(P, cut.bh, cut.rt, cut.split, DH);
+    if (!cut.sr.ok && tid == 0) atomicOr(P.status, kStatusBadLength);   // refused: zeros, nothing appended
+    if (!cut.sr.ok || cut.split >= cut.splits) {
+        if (!whole) tree_empty_partial(part, rows, DH, tid, kTreeThreads);
+        else for (int i = tid; i < rows * DH; i += kTreeThreads) Elem<T>::store(out + i, 0.f);
         return;
     }
 
@@ -214,9 +269,6 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
         __syncthreads();   // the stage may be filled again
     }
 
-    const bool whole = cut.splits == 1;
-    const size_t tile_index = (size_t)cut.bh * P.row_tiles + cut.rt;
-    float* part = whole ? nullptr : P.partials + (tile_index * P.splits + cut.split) * P.part_rows * ffa_tree_part_stride(DH);
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
         const int r = warp * RPW + i;
@@ -228,24 +280,10 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
         for (int x = 0; x < DPL; ++x) {
             const int d = lane + 32 * x;
             if (DH % 32 != 0 && d >= DH) break;
-            if (whole) Elem<T>::store(out + r * DH + d, L > 0.f ? acc[i][x] / L : 0.f);
+            if (whole) Elem<T>::store(out + r * DH + d, L == 0.f ? 0.f : acc[i][x] / L);
             else part[r * ffa_tree_part_stride(DH) + d] = acc[i][x];
         }
         if (!whole && lane == 0) part[r * ffa_tree_part_stride(DH) + DH] = m[i], part[r * ffa_tree_part_stride(DH) + DH + 1] = L;
-    }
-    if (whole) return;
-    // whoever arrives last merges; nobody waits (the fences are those of the decode kernels' merge)
-    __syncthreads();
-    int* ticket = P.tickets + cut.bh * kTreeTicketsPerPair + cut.rt;
-    if (tid == 0) {
-        __threadfence();
-        last = atomicAdd(ticket, 1) == cut.splits - 1;
-        __threadfence();
-    }
-    __syncthreads();
-    if (last) {
-        tree_merge<T, DH, false>(P.partials + tile_index * P.splits * P.part_rows * ffa_tree_part_stride(DH), cut.splits, P.part_rows, rows, out, tid, kTreeThreads);
-        if (tid == 0) *ticket = 0;
     }
 }
 

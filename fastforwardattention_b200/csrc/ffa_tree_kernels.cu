@@ -20,6 +20,16 @@ int with_rows(int rows, F&& f)
     return rows <= kTreeWarps ? f(ffa_tree_simt_kernel<float, DH, 1>) : f(ffa_tree_simt_kernel<float, DH, kManyRows>);
 }
 
+template <typename T, int DH, typename F>
+int with_copies(int tile_rows, F&& f)
+{
+    switch (umma_rep(tile_rows)) {
+        case 4: return f(ffa_tree_umma_kernel<T, DH, 4>);
+        case 2: return f(ffa_tree_umma_kernel<T, DH, 2>);
+        default: return f(ffa_tree_umma_kernel<T, DH, 1>);
+    }
+}
+
 int simt_rows(int rows) { return rows <= kTreeWarps ? kTreeWarps : kTreeWarps * kManyRows; }
 int simt_smem(int head_dim, int rows) { return simt_rows(rows) * head_dim * 4 + 4 * kTreeKeys * (head_dim * 4 + 16); }
 
@@ -68,12 +78,23 @@ int dispatch32(int head_dim, F&& f)
     });
 }
 
+template <typename T, int DH>
+int merge(const FfaTreeParams& P, cudaStream_t stream)
+{
+    const long long rows = (long long)P.B * P.H * P.groups * P.tokens;
+    return (int)launch_pdl(ffa_tree_merge_kernel<T, DH, sizeof(T) == 2>, (int)((rows + kMergeWarps - 1) / kMergeWarps), 32 * kMergeWarps, 0, 0, true, stream,
+                           P);
+}
+
 }  // namespace
 
 void ffa_k_tree_shape(int dtype, int head_dim, int rows, int* tile_rows, int* tile_keys, int* ctas_per_sm)
 {
     if (dtype == 0) *tile_rows = simt_rows(rows), *tile_keys = kTreeKeys, *ctas_per_sm = 2;
-    else *tile_rows = kUmmaRows, *tile_keys = kUmmaKeys, *ctas_per_sm = umma_ctas_per_sm(head_dim);
+    else {
+        const int tiles = (rows + kUmmaRows - 1) / kUmmaRows;   // of about equal height
+        *tile_rows = (rows + tiles - 1) / tiles, *tile_keys = kUmmaKeys, *ctas_per_sm = umma_ctas_per_sm(head_dim);
+    }
 }
 
 int ffa_k_tree_prepare(int dtype, int head_dim)
@@ -93,8 +114,13 @@ int ffa_k_tree_prepare(int dtype, int head_dim)
     return dispatch16(dtype, head_dim, [&](auto t, auto dh) -> int {
         using T = decltype(t);
         constexpr int DH = decltype(dh)::value;
-        return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(ffa_tree_umma_kernel<T, DH>), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         umma_smem(DH));
+        for (int rows : {32, 64, 128}) {
+            const int e = with_copies<T, DH>(rows, [&](auto kernel) {
+                return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, umma_smem(DH));
+            });
+            if (e != 0) return e;
+        }
+        return 0;
     });
 }
 
@@ -105,7 +131,8 @@ int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaSt
     if (dtype == 0)
         return dispatch32(head_dim, [&](auto dh) -> int {
             constexpr int DH = decltype(dh)::value;
-            return with_rows<DH>(rows, [&](auto kernel) { return (int)launch_pdl(kernel, grid, kTreeThreads, simt_smem(DH, rows), 0, true, stream, P); });
+            const int e = with_rows<DH>(rows, [&](auto kernel) { return (int)launch_pdl(kernel, grid, kTreeThreads, simt_smem(DH, rows), 0, true, stream, P); });
+            return e != 0 || P.splits == 1 ? e : merge<float, DH>(P, stream);
         });
     FfaTreeUmmaParams U;
     U.p = P;
@@ -121,7 +148,10 @@ int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaSt
     return dispatch16(dtype, head_dim, [&](auto t, auto dh) -> int {
         using T = decltype(t);
         constexpr int DH = decltype(dh)::value;
-        return (int)launch_pdl(ffa_tree_umma_kernel<T, DH>, grid, kUmmaThreads, umma_smem(DH), 0, true, stream, U);
+        const int r = with_copies<T, DH>(P.tile_rows, [&](auto kernel) {
+            return (int)launch_pdl(kernel, grid, kUmmaThreads, umma_smem(DH), 0, true, stream, U);
+        });
+        return r != 0 || P.splits == 1 ? r : merge<T, DH>(P, stream);
     });
 }
 

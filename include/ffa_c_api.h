@@ -186,7 +186,7 @@ int ffa_attention_paged(ffa_plan_t* plan, const void* q, const void* k, const vo
  * Statistics and sums are fp32; fp16 and bf16 weights are rounded to the tensors' type before they meet V, and the result once.
  * groups * tokens <= 1024.  page_table: NULL, or the paged caches of ffa_attention_paged.
  * scratch: ffa_tree_scratch_bytes(plan, groups, tokens, t) bytes of device memory (may be 0), 16-byte aligned, used by this call
- * only.  Like every call on a plan, calls are stream-ordered (the arrival counters are in the bound workspace). */
+ * only. */
 int ffa_tree_scratch_bytes(const ffa_plan_t* plan, int groups, int tokens, int t, size_t* bytes);
 int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
                        const unsigned char* tree, int tree_per_sample, int groups, int tokens, void* out, float softmax_scale,

@@ -35,7 +35,7 @@ def tree_attention(q, k, v, k_cache, v_cache, tree, scale, rows, first=None):
                 m = s.amax(-1, keepdim=True)
                 p = torch.where(see, (s - torch.where(m == -math.inf, 0.0, m)).exp(), 0.0)
                 total = p.sum(-1, keepdim=True)
-                p = torch.where(total > 0, p / total, 0.0)
+                p = torch.where(total == 0, 0.0, p / total)   # a NaN score makes its row NaN
                 # a token that a row does not see has no part in it, whatever its values: 0 * inf is not formed
                 o = torch.stack([p[t][see[t]] @ vals[see[t]] for t in range(T)])
                 a = torch.stack([p[t][see[t]] @ vals[see[t]].abs() for t in range(T)])

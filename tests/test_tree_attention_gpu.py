@@ -32,9 +32,9 @@ def setup(dt, B, H, G, D, n, T, L=None, seed=0, per_sample=True):
     return FastForwardAttn.adopt(kc, vc), kc, vc, q, k, v, tree
 
 
-def check(ffa, kc, vc, q, k, v, tree, rows, call, first=None, what=""):
+def check(ffa, kc, vc, q, k, v, tree, rows, call, first=None, what="", scale=None):
     kb, vb = kc.clone(), vc.clone()
-    want, bound = D64.tree_attention(q, k, v, kb, vb, tree, q.shape[-1] ** -0.5, rows, first)
+    want, bound = D64.tree_attention(q, k, v, kb, vb, tree, q.shape[-1] ** -0.5 if scale is None else scale, rows, first)
     out = call()
     D64.assert_within(out, want, bound, what)
     T = k.shape[2]
@@ -112,6 +112,27 @@ def test_a_visible_infinity_reaches_the_rows_that_see_it_and_no_others(dt):
     want, bound = D64.tree_attention(q, k, v, kc, vc, tree, D ** -0.5, [n])
     assert not torch.isfinite(want).all() and torch.isfinite(want[0, 0, 0]).all()
     D64.assert_within(ffa.tree_attention(q, k, v, tree, D ** -0.5, n), want, bound)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("row", [5, 64, 70, 250, 299])
+def test_a_broken_key_makes_the_rows_that_see_it_nan(dt, row):
+    """NaN in one element of a cached key (every row sees it), and in a drafted one (its descendants do)."""
+    D, T, n = 128, 9, 300
+    ffa, kc, vc, q, k, v, tree = setup(dt, 1, 2, 1, D, n, T, seed=row)
+    kc[0, 0, row, 77] = float("nan")
+    k[0, 1, 4, 3] = float("nan")
+    want, bound = D64.tree_attention(q, k, v, kc, vc, tree, D ** -0.5, [n])
+    assert torch.isnan(want[0, 0]).all() and torch.isnan(want[0, 1, 4]).all() and torch.isfinite(want[0, 1, 0]).all()
+    D64.assert_within(ffa.tree_attention(q, k, v, tree, D ** -0.5, n), want, bound)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
+def test_any_scale(dt, scale):
+    D, T, n = 64, 30, 200
+    ffa, kc, vc, q, k, v, tree = setup(dt, 1, 2, 2, D, n, T, seed=41)
+    check(ffa, kc, vc, q, k, v, tree, [n], lambda: ffa.tree_attention(q, k, v, tree, scale, n), scale=scale)
 
 
 @pytest.mark.parametrize("dt", DTYPES)
