@@ -129,8 +129,15 @@ struct FfaAcceptParams {
     const int* page_table;
     int max_pages, page_rows;
 };
-// query rows per CTA, key rows per tile and resident CTAs per SM of the kernel that takes this type and number of query rows
-void ffa_k_tree_shape(int dtype, int head_dim, int rows, int* tile_rows, int* tile_keys, int* ctas_per_sm);
+// How a tree attention is cut: query rows per CTA, tiles of them, rows of a partial result, keys per tile, and what the choice of the
+// number of splits needs to know of the kernel that takes this type and number of query rows: resident CTAs per SM, and the time that
+// a CTA alone on an SM takes for a tile.
+struct FfaTreeShape {
+    int tile_rows, row_tiles, part_rows, tile_keys, ctas_per_sm;
+    double tile_us;
+    int splits;
+};
+void ffa_k_tree_shape(int dtype, int head_dim, int rows, FfaTreeShape* shape);
 int ffa_k_tree_prepare(int dtype, int head_dim);
 int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaStream_t stream);
 int ffa_k_tree_accept(const FfaAcceptParams& P, cudaStream_t stream);

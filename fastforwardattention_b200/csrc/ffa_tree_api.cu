@@ -9,39 +9,36 @@
 
 namespace {
 
-// The cut of a tree attention: tiles of query rows per pair, and CTAs per (pair, tile of query rows).
-struct TreeShape {
-    int tile_rows, row_tiles, part_rows, splits;
-};
-
-// A CTA's time is its key tiles plus a fixed part (start, first tile, epilogue: a few tiles' worth), and more for the merge when a
-// pair is split.  All CTAs of a full wave share HBM; a CTA that is nearly alone still takes a tile every third of a microsecond.  The
-// number of splits is the one with the smallest sum over the waves.
-TreeShape tree_shape(const ffa_plan* p, int groups, int tokens, int t)
+// A CTA's time is its key tiles plus a fixed part (start, first tile, epilogue), and more when a pair is split (partial results and
+// their merge).  The CTAs of a wave share HBM, and a tile takes each of them a certain time however few they are.  The number of
+// splits is the one with the smallest sum over the waves.  Measured with 1 / 2 / 4 / 7 / 9 / 10 / 18 splits: bf16 x 128, 32 pairs, 16000
+// tokens, 8 drafted: 190 / 102 / 56 / 47 / 50 / 64 / 54 us (7 is taken); 16 pairs, 32 K tokens, 132 query rows (9 is taken): 447 / 235 / 129 / 95 /
+// 83 / 116 / 96 us.
+FfaTreeShape tree_shape(const ffa_plan* p, int groups, int tokens, int t)
 {
-    TreeShape s;
-    const int rows = groups * tokens;
-    int tile_keys, cps;
-    ffa_k_tree_shape(p->dtype, p->Dh, rows, &s.tile_rows, &tile_keys, &cps);
-    s.row_tiles = (rows + s.tile_rows - 1) / s.tile_rows;
-    s.part_rows = rows < s.tile_rows ? rows : s.tile_rows;
-    const long long items = (long long)p->B * p->H * s.row_tiles, slots = (long long)p->sms * cps;
-    const long long tiles = (t + tile_keys - 1) / tile_keys + (tokens + tile_keys - 1) / tile_keys;
-    const double tile_us = 2.0 * tile_keys * p->Dh * ffa_elem_size(p->dtype) / 6.6e6;   // of the whole device's HBM bandwidth
+    FfaTreeShape s;
+    ffa_k_tree_shape(p->dtype, p->Dh, groups * tokens, &s);
+    const long long items = (long long)p->B * p->H * s.row_tiles, slots = (long long)p->sms * s.ctas_per_sm;
+    const long long tiles = (t + s.tile_keys - 1) / s.tile_keys + (tokens + s.tile_keys - 1) / s.tile_keys;
+    const double share_us = 2.0 * s.tile_keys * p->Dh * ffa_elem_size(p->dtype) / 6.0e6;   // a tile at the whole device's bandwidth
     double best = 0;
     s.splits = 1;
     for (long long splits = 1; splits <= tiles && splits <= kTreeMaxSplits; ++splits) {
         const long long ctas = items * splits, full = ctas / slots, rest = ctas % slots;
         const double run = (double)((tiles + splits - 1) / splits);
-        const double fixed = 3.0 + (splits > 1 ? 1.5 + 0.1 * splits : 0.0);
-        auto wave = [&](long long n) { return n == 0 ? 0.0 : run * (n * tile_us > 0.35 ? n * tile_us : 0.35) + fixed; };
+        const double fixed = 5.0 + (splits > 1 ? 2.0 + 0.05 * splits : 0.0);
+        auto wave = [&](long long n) {
+            // CTAs that share an SM slow one another down by about half of what they would without overlap
+            const double crowd = s.tile_us * (n > p->sms ? 0.5 + 0.5 * n / p->sms : 1.0), shared = n * share_us;
+            return n == 0 ? 0.0 : run * (crowd > shared ? crowd : shared) + fixed;
+        };
         const double us = full * wave(slots) + wave(rest);
         if (splits == 1 || us < best) best = us, s.splits = (int)splits;
     }
     return s;
 }
 
-size_t tree_partials_bytes(const ffa_plan* p, const TreeShape& s)
+size_t tree_partials_bytes(const ffa_plan* p, const FfaTreeShape& s)
 {
     if (s.splits <= 1) return 0;
     return (size_t)p->B * p->H * s.row_tiles * s.splits * s.part_rows * ffa_tree_part_stride(p->Dh) * sizeof(float);
@@ -99,7 +96,7 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
     if (r != FFA_OK) return r;
     if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
     if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
-    const TreeShape s = tree_shape(plan, groups, tokens, t);
+    const FfaTreeShape s = tree_shape(plan, groups, tokens, t);
     const size_t need = tree_partials_bytes(plan, s);
     if (need > 0 && (scratch == nullptr || scratch_bytes < need))
         return ffa_fail(FFA_ERR_WORKSPACE, "scratch of %zu bytes, need %zu (ffa_tree_scratch_bytes)", scratch ? scratch_bytes : (size_t)0, need);

@@ -12,8 +12,7 @@
 namespace ffa_dev {
 
 constexpr int kTreeThreads = 256;
-constexpr int kTreeWarps = kTreeThreads / 32;
-constexpr int kTreeKeys = 32;   // keys per tile of the CUDA-core kernel: one per lane
+constexpr int kTreeKeys = 64;   // keys per tile of the CUDA-core kernel
 
 // What one CTA of a tree attention works on: a pair, a tile of its query rows, a run of its key tiles.  Key tiles are
 // whole tiles of the cache (KEYS rows, aligned to KEYS) followed by tiles of drafted tokens; a sample with fewer tiles
@@ -41,17 +40,25 @@ struct TreeCut {
     __device__ __forceinline__ bool owns_new_tokens() const { return split == splits - 1 && rt == 0; }
 };
 
-// k and v of the drafted tokens -> rows n..n+tokens-1 of the cache, by `threads` threads
-__device__ __forceinline__ void tree_append(const FfaTreeParams& P, int bh, int row, int rowb, int tid, int threads)
+// k and v of the drafted tokens -> rows n..n+tokens-1 of the cache: vectors first, first + step, ... of the tokens' 16-byte vectors
+__device__ __forceinline__ void tree_append(const FfaTreeParams& P, int bh, int row, int rowb, int first, int step)
 {
-    const int vpr = rowb / 16;
-    const unsigned char* ks = static_cast<const unsigned char*>(P.k) + (size_t)bh * P.tokens * rowb;
-    const unsigned char* vs = static_cast<const unsigned char*>(P.v) + (size_t)bh * P.tokens * rowb;
-    for (int i = tid; i < P.tokens * vpr; i += threads) {
-        const int j = i / vpr, c = i - j * vpr;
-        const size_t to = cache_row_offset(P, bh, row + j, rowb) + c * 16;
-        *reinterpret_cast<uint4*>(static_cast<unsigned char*>(P.k_cache) + to) = *reinterpret_cast<const uint4*>(ks + (size_t)i * 16);
-        *reinterpret_cast<uint4*>(static_cast<unsigned char*>(P.v_cache) + to) = *reinterpret_cast<const uint4*>(vs + (size_t)i * 16);
+    const int vpr = rowb / 16, total = P.tokens * vpr;
+    const uint4* ks = static_cast<const uint4*>(P.k) + (size_t)bh * total;
+    const uint4* vs = static_cast<const uint4*>(P.v) + (size_t)bh * total;
+    for (int i0 = first; i0 < total; i0 += 4 * step) {
+        uint4 x[4], y[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            if (i0 + n * step < total) x[n] = ks[i0 + n * step], y[n] = vs[i0 + n * step];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const int i = i0 + n * step;
+            if (i >= total) break;
+            const size_t to = cache_row_offset(P, bh, row + i / vpr, rowb) + (i % vpr) * 16;
+            *reinterpret_cast<uint4*>(static_cast<unsigned char*>(P.k_cache) + to) = x[n];
+            *reinterpret_cast<uint4*>(static_cast<unsigned char*>(P.v_cache) + to) = y[n];
+        }
     }
 }
 
@@ -133,164 +140,196 @@ __global__ void __launch_bounds__(32 * kMergeWarps) ffa_tree_merge_kernel(const 
     }
 }
 
-// CUDA-core kernel.  8 warps; a warp owns RPW query rows, a lane one key of the tile: the scores of a row live in one warp, so
-// the softmax needs shuffles only.  K and V tiles (32 keys) come through a two-stage cp.async ring with 16 bytes of padding per
-// row (a quarter warp's 16-byte reads of 8 different rows then hit different banks).  Rows outside the valid range are
-// zero-filled, never read, so that what a cache holds behind its last row cannot reach the result.
-template <typename T, int DH, int RPW>
+// CUDA-core kernel (fp32).  A CTA of 16 x 16 threads takes 16 * RT query rows and tiles of 64 keys.
+//   S   a thread computes RT rows x 4 keys: per 16 bytes of the head dimension RT + 4 shared-memory reads feed 8 * RT packed FMAs
+//       (rows of K are padded by 16 bytes: 8 lanes' 16-byte reads of 8 rows then hit different banks; a warp reads two rows of Q)
+//   P   through shared memory, transposed, the groups of rows XORed with the key so that neither side has bank conflicts
+//   O   a thread keeps RT rows x DH / 16 columns
+// K and V have one buffer each: V of a tile arrives while S is computed, K of the next one while O is.  Rows outside the valid range
+// are zero-filled, never read, so that what a cache holds behind its last row cannot reach the result.  What bounds it: HBM for a few rows,
+// fp32 FMAs from about 16 on.
+template <int DH, int RT>
 __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTreeParams P)
 {
-    constexpr int BM = kTreeWarps * RPW, BN = kTreeKeys, ROWB = DH * (int)sizeof(T), PITCH = ROWB + 16, VPR = ROWB / 16;
-    constexpr int EPV = Elem<T>::EPV, DPL = (DH + 31) / 32;
+    constexpr int BM = 16 * RT, BN = kTreeKeys, VPR = DH / 4, KP = DH + 4, XV = (VPR + 15) / 16;
     extern __shared__ __align__(128) unsigned char smem[];
-    float* qs = reinterpret_cast<float*>(smem);                       // [BM][DH], scaled
-    unsigned char* ring = smem + (size_t)BM * DH * 4;                  // [2 stages][K | V][BN][PITCH]
+    float* qs = reinterpret_cast<float*>(smem);   // [BM][DH], scaled
+    float* ks = qs + BM * DH;                      // [BN][KP]
+    float* vs = ks + BN * KP;                      // [BN][DH]
+    float* ps = vs + BN * DH;                      // [BN][16 groups of RT]
 
     pdl_release();
     pdl_wait();
     const TreeCut<BN> cut(P);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int R = P.groups * P.tokens, row0 = cut.rt * BM, rows = min(BM, R - row0);
     const bool whole = P.splits == 1;
-    T* out = static_cast<T*>(P.out) + ((size_t)cut.bh * R + row0) * DH;
+    float* out = static_cast<float*>(P.out) + ((size_t)cut.bh * R + row0) * DH;
     float* part = whole ? nullptr : tree_partial(P, cut.bh, cut.rt, cut.split, DH);
     if (!cut.sr.ok && tid == 0) atomicOr(P.status, kStatusBadLength);   // refused: zeros, nothing appended
     if (!cut.sr.ok || cut.split >= cut.splits) {
         if (!whole) tree_empty_partial(part, rows, DH, tid, kTreeThreads);
-        else for (int i = tid; i < rows * DH; i += kTreeThreads) Elem<T>::store(out + i, 0.f);
+        else for (int i = tid; i < rows * DH; i += kTreeThreads) out[i] = 0.f;
         return;
     }
 
-    auto load_tile = [&](int u, int stage) {
+    auto load = [&](int u, bool is_v) {
         const bool cached = u < cut.cache_tiles;
         const int base = (cached ? cut.c0 + u : u - cut.cache_tiles) * BN;
         const int lo = cached ? cut.sr.first : 0, hi = cached ? cut.sr.row : P.tokens;
-        const size_t off = cached ? cache_row_offset(P, cut.bh, base, ROWB) : ((size_t)cut.bh * P.tokens + base) * ROWB;
-        const unsigned char* ks = static_cast<const unsigned char*>(cached ? P.k_cache : P.k) + off;
-        const unsigned char* vs = static_cast<const unsigned char*>(cached ? P.v_cache : P.v) + off;
-        const uint32_t dst = smem_u32(ring) + stage * 2 * BN * PITCH;
+        const size_t off = cached ? cache_row_offset(P, cut.bh, base, DH * 4) : ((size_t)cut.bh * P.tokens + base) * (DH * 4);
+        const unsigned char* src = static_cast<const unsigned char*>(is_v ? (cached ? P.v_cache : P.v) : (cached ? P.k_cache : P.k));
+        const uint32_t dst = smem_u32(is_v ? vs : ks);
+        const int pitch = (is_v ? DH : KP) * 4;
         for (int i = tid; i < BN * VPR; i += kTreeThreads) {
             const int r = i / VPR, c = i - r * VPR;
             const bool in = base + r >= lo && base + r < hi;
-            const size_t from = in ? (size_t)i * 16 : 0;
-            cp_async_16_or_zero(dst + r * PITCH + c * 16, in ? ks + from : static_cast<const unsigned char*>(P.k), in ? 16u : 0u);
-            cp_async_16_or_zero(dst + (BN + r) * PITCH + c * 16, in ? vs + from : static_cast<const unsigned char*>(P.v), in ? 16u : 0u);
+            cp_async_16_or_zero(dst + r * pitch + c * 16, in ? src + off + (size_t)i * 16 : static_cast<const unsigned char*>(P.k), in ? 16u : 0u);
         }
         cp_async_commit();
     };
 
-    load_tile(cut.u0, 0);
+    load(cut.u0, false);
+    load(cut.u0, true);
     {
-        const T* q = static_cast<const T*>(P.q) + ((size_t)cut.bh * R + row0) * DH;
-        for (int i = tid; i < BM * DH; i += kTreeThreads) qs[i] = i < rows * DH ? Elem<T>::to_float(q[i]) * P.scale : 0.f;
+        const float* q = static_cast<const float*>(P.q) + ((size_t)cut.bh * R + row0) * DH;
+        for (int i = tid; i < BM * DH; i += kTreeThreads) qs[i] = i < rows * DH ? q[i] * P.scale : 0.f;
     }
-    if (cut.owns_new_tokens()) tree_append(P, cut.bh, cut.sr.row, ROWB, tid, kTreeThreads);
 
-    float m[RPW], l[RPW], acc[RPW][DPL];
+    float m[RT], l[RT];
+    float2 o[RT][XV][2];
 #pragma unroll
-    for (int i = 0; i < RPW; ++i) {
+    for (int i = 0; i < RT; ++i) {
         m[i] = -CUDART_INF_F, l[i] = 0.f;
 #pragma unroll
-        for (int x = 0; x < DPL; ++x) acc[i][x] = 0.f;
+        for (int x = 0; x < XV; ++x) o[i][x][0] = o[i][x][1] = make_float2(0.f, 0.f);
     }
-    const bool busy = warp * RPW < rows;   // this warp has query rows
+    const bool busy = (ty & ~1) * RT < rows;   // this warp has query rows
     for (int u = cut.u0; u < cut.u1; ++u) {
-        const int stage = (u - cut.u0) & 1;
-        if (u + 1 < cut.u1) {
-            load_tile(u + 1, stage ^ 1);
-            cp_async_wait<1>();
-        } else {
-            cp_async_wait<0>();
-        }
+        const bool cached = u < cut.cache_tiles;
+        const int base = (cached ? cut.c0 + u : u - cut.cache_tiles) * BN;
+        cp_async_wait<1>();   // K is here, V may be on its way
         __syncthreads();
         if (busy) {
-            const unsigned char* kt = ring + (size_t)stage * 2 * BN * PITCH;
-            const unsigned char* vt = kt + BN * PITCH;
-            const bool cached = u < cut.cache_tiles;
-            const int key = (cached ? cut.c0 + u : u - cut.cache_tiles) * BN + lane;
-            float s[RPW];
+            float2 acc[RT][4];
 #pragma unroll
-            for (int i = 0; i < RPW; ++i) s[i] = 0.f;
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) acc[i][n] = make_float2(0.f, 0.f);
 #pragma unroll 4
             for (int c = 0; c < VPR; ++c) {
-                float kf[EPV];
-                Elem<T>::unpack(*reinterpret_cast<const uint4*>(kt + lane * PITCH + c * 16), kf);
+                float4 q4[RT], k4[4];
 #pragma unroll
-                for (int i = 0; i < RPW; ++i) {
-                    const float* qr = qs + (warp * RPW + i) * DH + c * EPV;
+                for (int i = 0; i < RT; ++i) q4[i] = *reinterpret_cast<const float4*>(qs + (ty * RT + i) * DH + 4 * c);
 #pragma unroll
-                    for (int e = 0; e < EPV; e += 4) {
-                        const float4 q4 = *reinterpret_cast<const float4*>(qr + e);
-                        s[i] = fmaf(q4.x, kf[e], s[i]), s[i] = fmaf(q4.y, kf[e + 1], s[i]);
-                        s[i] = fmaf(q4.z, kf[e + 2], s[i]), s[i] = fmaf(q4.w, kf[e + 3], s[i]);
+                for (int n = 0; n < 4; ++n) k4[n] = *reinterpret_cast<const float4*>(ks + (tx + 16 * n) * KP + 4 * c);
+#pragma unroll
+                for (int i = 0; i < RT; ++i)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        acc[i][n] = __ffma2_rn(make_float2(q4[i].x, q4[i].y), make_float2(k4[n].x, k4[n].y), acc[i][n]);
+                        acc[i][n] = __ffma2_rn(make_float2(q4[i].z, q4[i].w), make_float2(k4[n].z, k4[n].w), acc[i][n]);
                     }
+            }
+            float p[4][RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const int r = row0 + ty * RT + i;
+                const unsigned char* sees = P.tree + ((size_t)(P.tree_per_sample ? cut.b : 0) * P.tokens + r % P.tokens) * P.tokens;
+                float s[4], top = -CUDART_INF_F;
+                bool see[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const int key = base + tx + 16 * n;
+                    see[n] = r < R && (cached ? key >= cut.sr.first && key < cut.sr.row : key < P.tokens && sees[key] != 0);
+                    s[n] = see[n] ? acc[i][n].x + acc[i][n].y : -CUDART_INF_F;
+                    top = fmaxf(top, s[n]);
                 }
+#pragma unroll
+                for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+                top = fmaxf(m[i], top);
+                const float ref = top == -CUDART_INF_F ? 0.f : top;   // nothing seen so far: every weight is 0, not NaN
+                const float corr = expf(m[i] - ref);
+                m[i] = top;
+                l[i] *= corr;   // this thread's keys; the threads are added at the end
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    p[n][i] = see[n] ? expf(s[n] - ref) : 0.f;
+                    l[i] += p[n][i];
+                }
+#pragma unroll
+                for (int x = 0; x < XV; ++x)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) o[i][x][h] = __fmul2_rn(o[i][x][h], make_float2(corr, corr));
             }
 #pragma unroll
-            for (int i = 0; i < RPW; ++i) {
-                const int r = row0 + warp * RPW + i;
-                bool see = r < R;
-                if (cached) {
-                    see = see && key >= cut.sr.first && key < cut.sr.row;
-                } else {
-                    const int t = r % P.tokens;
-                    see = see && key < P.tokens &&
-                          P.tree[((size_t)(P.tree_per_sample ? cut.b : 0) * P.tokens + t) * P.tokens + key] != 0;
-                }
-                s[i] = see ? s[i] : -CUDART_INF_F;
-                float mx = s[i];
+            for (int n = 0; n < 4; ++n) {
+                const int key = tx + 16 * n;
+                float* to = ps + key * BM + (ty ^ (key & 15)) * RT;
 #pragma unroll
-                for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                mx = fmaxf(m[i], mx);
-                const float base = mx == -CUDART_INF_F ? 0.f : mx;   // nothing seen so far: every weight is 0, not NaN
-                const float corr = expf(m[i] - base);
-                m[i] = mx;
-                s[i] = see ? expf(s[i] - base) : 0.f;
-                l[i] = l[i] * corr + s[i];   // this lane's keys; the lanes are added at the end
-#pragma unroll
-                for (int x = 0; x < DPL; ++x) acc[i][x] *= corr;
-            }
-#pragma unroll 4
-            for (int j = 0; j < BN; ++j) {
-                const T* vr = reinterpret_cast<const T*>(vt + j * PITCH);
-                float vf[DPL];
-#pragma unroll
-                for (int x = 0; x < DPL; ++x) vf[x] = (DH % 32 == 0 || lane + 32 * x < DH) ? Elem<T>::to_float(vr[lane + 32 * x]) : 0.f;
-#pragma unroll
-                for (int i = 0; i < RPW; ++i) {
-                    const float pj = __shfl_sync(0xffffffffu, s[i], j);
-                    if (pj != 0.f) {   // a hidden token has no part in the row, whatever its values
-#pragma unroll
-                        for (int x = 0; x < DPL; ++x) acc[i][x] = fmaf(pj, vf[x], acc[i][x]);
-                    }
-                }
+                for (int i = 0; i < RT; ++i) to[i] = p[n][i];
             }
         }
-        __syncthreads();   // the stage may be filled again
+        cp_async_wait<0>();
+        __syncthreads();   // P is written, V is here, K's buffer is free
+        if (u + 1 < cut.u1) load(u + 1, false);
+        if (busy) {
+            auto values = [&](auto guard_tag) {
+                constexpr bool kGuard = decltype(guard_tag)::value;
+#pragma unroll 4
+                for (int key = 0; key < BN; ++key) {
+                    float pr[RT];
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) pr[i] = ps[key * BM + (ty ^ (key & 15)) * RT + i];
+#pragma unroll
+                    for (int x = 0; x < XV; ++x) {
+                        const int c = tx + 16 * x;
+                        if (VPR % 16 != 0 && c >= VPR) break;
+                        const float4 v4 = *reinterpret_cast<const float4*>(vs + key * DH + 4 * c);
+#pragma unroll
+                        for (int i = 0; i < RT; ++i) {
+                            if (kGuard && pr[i] == 0.f) continue;   // a hidden token has no part in the row, whatever its values
+                            o[i][x][0] = __ffma2_rn(make_float2(pr[i], pr[i]), make_float2(v4.x, v4.y), o[i][x][0]);
+                            o[i][x][1] = __ffma2_rn(make_float2(pr[i], pr[i]), make_float2(v4.z, v4.w), o[i][x][1]);
+                        }
+                    }
+                }
+            };
+            if (cached) values(std::false_type{});
+            else values(std::true_type{});
+        }
+        __syncthreads();   // V's buffer and P are free
+        if (u + 1 < cut.u1) load(u + 1, true);
     }
 
 #pragma unroll
-    for (int i = 0; i < RPW; ++i) {
-        const int r = warp * RPW + i;
-        if (r >= rows) break;
+    for (int i = 0; i < RT; ++i) {
+        const int r = ty * RT + i;
         float L = l[i];
 #pragma unroll
-        for (int off = 16; off >= 1; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        for (int off = 8; off >= 1; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+        if (r >= rows) continue;
+        const float inv = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+        float* to = whole ? out + (size_t)r * DH : part + (size_t)r * ffa_tree_part_stride(DH);
 #pragma unroll
-        for (int x = 0; x < DPL; ++x) {
-            const int d = lane + 32 * x;
-            if (DH % 32 != 0 && d >= DH) break;
-            if (whole) Elem<T>::store(out + r * DH + d, L == 0.f ? 0.f : acc[i][x] / L);
-            else part[r * ffa_tree_part_stride(DH) + d] = acc[i][x];
+        for (int x = 0; x < XV; ++x) {
+            const int c = tx + 16 * x;
+            if (VPR % 16 != 0 && c >= VPR) break;
+            *reinterpret_cast<float4*>(to + 4 * c) = make_float4(o[i][x][0].x * inv, o[i][x][0].y * inv, o[i][x][1].x * inv, o[i][x][1].y * inv);
         }
-        if (!whole && lane == 0) part[r * ffa_tree_part_stride(DH) + DH] = m[i], part[r * ffa_tree_part_stride(DH) + DH + 1] = L;
+        if (!whole && tx == 0) to[DH] = m[i], to[DH + 1] = L;
     }
+    // the drafted tokens go to the cache behind the last read of this CTA, a share from each of the pair's CTAs
+    const int ctas = cut.splits * P.row_tiles, mine = cut.split * P.row_tiles + cut.rt;
+    tree_append(P, cut.bh, cut.sr.row, DH * 4, mine * kTreeThreads + tid, ctas * kTreeThreads);
 }
 
 // Rows n + path[i] -> n + i of every pair, in place.  A thread owns one 16-byte column of K or V and walks the path: indices
 // increase, so path[i] >= i and a row is read before anything is written to it (eight rows are read, then eight written).
 __global__ void __launch_bounds__(256) ffa_tree_accept_kernel(const FfaAcceptParams P)
 {
+    pdl_release();
+    pdl_wait();
     const int bh = blockIdx.x, b = bh / P.H;
     const int vpr = P.row_bytes / 16;
     const int* path = P.path + (size_t)b * P.path_len;

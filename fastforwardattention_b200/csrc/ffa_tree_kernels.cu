@@ -10,14 +10,22 @@ using namespace ffa_dev;
 
 namespace {
 
-// query rows per warp of the CUDA-core kernel: a pair with at most 8 rows takes one per warp (with four, a quarter of the warps would
-// have them all)
-constexpr int kManyRows = 4;
-
+// query rows per thread of the CUDA-core kernel (16 threads deep): as few as hold all rows, at most four
+int simt_rt(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 template <int DH, typename F>
 int with_rows(int rows, F&& f)
 {
-    return rows <= kTreeWarps ? f(ffa_tree_simt_kernel<float, DH, 1>) : f(ffa_tree_simt_kernel<float, DH, kManyRows>);
+    switch (simt_rt(rows)) {
+        case 1: return f(ffa_tree_simt_kernel<DH, 1>);
+        case 2: return f(ffa_tree_simt_kernel<DH, 2>);
+        default: return f(ffa_tree_simt_kernel<DH, 4>);
+    }
+}
+constexpr int kSmemPerSm = 228 * 1024;
+int simt_smem(int head_dim, int rows)
+{
+    const int bm = 16 * simt_rt(rows);
+    return 4 * (bm * head_dim + kTreeKeys * (head_dim + 4) + kTreeKeys * head_dim + kTreeKeys * bm);
 }
 
 template <typename T, int DH, typename F>
@@ -29,9 +37,6 @@ int with_copies(int tile_rows, F&& f)
         default: return f(ffa_tree_umma_kernel<T, DH, 1>);
     }
 }
-
-int simt_rows(int rows) { return rows <= kTreeWarps ? kTreeWarps : kTreeWarps * kManyRows; }
-int simt_smem(int head_dim, int rows) { return simt_rows(rows) * head_dim * 4 + 4 * kTreeKeys * (head_dim * 4 + 16); }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -88,13 +93,22 @@ int merge(const FfaTreeParams& P, cudaStream_t stream)
 
 }  // namespace
 
-void ffa_k_tree_shape(int dtype, int head_dim, int rows, int* tile_rows, int* tile_keys, int* ctas_per_sm)
+void ffa_k_tree_shape(int dtype, int head_dim, int rows, FfaTreeShape* s)
 {
-    if (dtype == 0) *tile_rows = simt_rows(rows), *tile_keys = kTreeKeys, *ctas_per_sm = 2;
-    else {
+    if (dtype == 0) {
+        s->tile_rows = 16 * simt_rt(rows), s->tile_keys = kTreeKeys;
+        const int fit = kSmemPerSm / (simt_smem(head_dim, rows) + 1024);
+        s->ctas_per_sm = fit > 4 ? 4 : fit;
+        // S and O of a tile: 4 * rows * keys * Dh flops at about 55 % of an SM's 128 FMAs a cycle, and two memory latencies
+        s->tile_us = 0.6 + 4.0 * s->tile_rows * kTreeKeys * head_dim / (2 * 128 * 0.55 * 1900);
+    } else {
         const int tiles = (rows + kUmmaRows - 1) / kUmmaRows;   // of about equal height
-        *tile_rows = (rows + tiles - 1) / tiles, *tile_keys = kUmmaKeys, *ctas_per_sm = umma_ctas_per_sm(head_dim);
+        s->tile_rows = (rows + tiles - 1) / tiles, s->tile_keys = kUmmaKeys, s->ctas_per_sm = umma_ctas_per_sm(head_dim);
+        // measured, one CTA to an SM: the chain S - softmax - O per tile, longer for Dh 256 by its products
+        s->tile_us = head_dim > 128 ? 1.5 : umma_rep(s->tile_rows) == 1 ? 0.9 : 0.75;
     }
+    s->row_tiles = (rows + s->tile_rows - 1) / s->tile_rows;
+    s->part_rows = rows < s->tile_rows ? rows : s->tile_rows;
 }
 
 int ffa_k_tree_prepare(int dtype, int head_dim)
@@ -102,7 +116,7 @@ int ffa_k_tree_prepare(int dtype, int head_dim)
     if (dtype == 0)
         return dispatch32(head_dim, [&](auto dh) -> int {
             constexpr int DH = decltype(dh)::value;
-            for (int rows : {1, kTreeMaxRows}) {
+            for (int rows : {16, 32, 64}) {
                 const int e = with_rows<DH>(rows, [&](auto kernel) {
                     return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, simt_smem(DH, rows));
                 });
@@ -158,6 +172,5 @@ int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaSt
 int ffa_k_tree_accept(const FfaAcceptParams& P, cudaStream_t stream)
 {
     const int threads = (2 * P.row_bytes / 16 + 31) / 32 * 32;
-    ffa_tree_accept_kernel<<<(unsigned)(P.B * P.H), threads, 0, stream>>>(P);
-    return (int)cudaGetLastError();
+    return (int)launch_pdl(ffa_tree_accept_kernel, P.B * P.H, threads, 0, 0, true, stream, P);
 }
