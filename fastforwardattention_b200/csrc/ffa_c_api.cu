@@ -633,14 +633,6 @@ int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void
         return fail(FFA_ERR_WORKSPACE, "this shape needs the streaming pruning kernel: bind a workspace sized with with_scores = 1");
 
     ffa_launch_t L;
-    // accumulating steps merge split pairs through global memory, whose last arriver adds the weights: the cut is the one of
-    // a plan without the cluster merge
-    ffa_plan without_clusters;
-    if (weighs) {
-        without_clusters = *plan;
-        without_clusters.cluster_merge = 0;
-        plan = &without_clusters;
-    }
     // the streaming kernel never lets a tile straddle a page: tiles are powers of two that divide it
     int r = fit_launch(plan, cap, twopass ? 1 : 2, &L, /*pow2_tiles=*/paged);
     if (r != FFA_OK) return r;
@@ -659,6 +651,7 @@ int run_step(ffa_plan_t* plan, const void* q, const void* k, const void* v, void
         // (pairs with more than 8 parts: whole clusters of 8, the cluster leaders merge through global memory)
         r = fit_clusters(plan, cap, paged, &L, &P.cluster);
         if (r != FFA_OK) return r;
+        if (weighs && L.parts_per_bh > kMaxClusterCtas) P.cluster = 0;   // more than one cluster per pair: the last arriver adds the weights
         P.tile_rows = L.tile_rows, P.stages = L.stages, P.grid = L.grid;
         P.units_per_bh = cap / L.tile_rows + 1;
         P.parts_per_bh = L.parts_per_bh;

@@ -183,8 +183,15 @@ int ffa_k_decode_onepass(int dtype, int head_dim, const FfaStepParams& P, int th
         constexpr int DH = decltype(dh)::value;
         // rows the step streams: at most t of every pair (per-sample lengths: t is their bound)
         const bool overlap = 2.0 * P.B * P.H * P.t * DH * sizeof(T) < kPdlBelowBytes;
-        if (P.weights != nullptr)
-            return (int)launch_pdl(ffa_stream_kernel<T, DH, true>, P.grid, threads, smem, 0, overlap, stream, P);
+        if (P.weights != nullptr) {
+            if (P.cluster > 1) {
+                if (launch_pdl(ffa_stream_kernel<T, DH, true>, P.grid, threads, smem, P.cluster, overlap, stream, P) == cudaSuccess) return 0;
+                (void)cudaGetLastError();   // as below
+            }
+            FfaStepParams Q = P;
+            Q.cluster = 0;
+            return (int)launch_pdl(ffa_stream_kernel<T, DH, true>, Q.grid, threads, smem, 0, overlap, stream, Q);
+        }
         if (P.cluster > 1) {   // the CTAs that share a (batch, head) as one thread-block cluster
             if (launch_pdl(ffa_stream_kernel<T, DH, false>, P.grid, threads, smem, P.cluster, overlap, stream, P) == cudaSuccess) return 0;
             // a cluster shape this device cannot co-schedule: the same cut runs without clusters,

@@ -153,9 +153,8 @@ struct FfaEvictParams {
     int B, H, Lmax, max_rows, keep, recent, first, row_bytes;
     int* status;
 };
-int ffa_k_evict_smem(int max_rows);
 int ffa_k_evict_prepare(int max_smem);
-int ffa_k_evict(const FfaEvictParams& P, int smem, cudaStream_t stream);
+int ffa_k_evict(const FfaEvictParams& P, cudaStream_t stream);   // one launch, two when more than one row of a pair may have to go
 
 // Selection over beams and vocabulary (ffa_beam_select).
 struct FfaBeamParams {

@@ -30,14 +30,15 @@ int ffa_evict(ffa_plan_t* plan, void* k_cache, void* v_cache, float* weights, in
         return ffa_fail(FFA_ERR_RANGE, "need 0 <= recent (%d), 0 <= first (%d), recent + first <= keep (%d)", recent, first, keep);
     if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
     if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
+    if ((long long)plan->B * plan->H * ((keep + 31) / 32) >= (1LL << 31)) return ffa_fail(FFA_ERR_RANGE, "sizes exceed int range");
     FfaEvictParams P;
     std::memset(&P, 0, sizeof(P));
     P.k_cache = k_cache, P.v_cache = v_cache, P.weights = weights, P.positions = positions, P.rows = rows, P.kept = kept;
     P.B = plan->B, P.H = plan->H, P.Lmax = plan->Lmax, P.max_rows = max_rows, P.keep = keep, P.recent = recent, P.first = first;
     P.row_bytes = plan->Dh * ffa_elem_size(plan->dtype), P.status = plan->status;
-    const int r = ffa_k_evict(P, ffa_k_evict_smem(max_rows), static_cast<cudaStream_t>(stream));
+    const int r = ffa_k_evict(P, static_cast<cudaStream_t>(stream));
     if (r != 0) return ffa_cuda_fail(r, "eviction launch");
-    ffa_count_launches(1);
+    ffa_count_launches(max_rows > keep + 1 ? 2 : 1);
     return FFA_OK;
 }
 

@@ -67,8 +67,34 @@ __device__ __forceinline__ void merge_partials(const FfaStepParams& P, uint32_t 
 // owns a row: 16-byte shared-memory reads, fp32 FMAs, butterfly sum.  Each group keeps its
 // own online-softmax state, so the row loop has no CTA-level synchronisation at all.
 // kWeigh: the step also accumulates every attended row's probability into P.weights.  A row's score goes to the score scratch as
-// it is computed (4 bytes a row, L2-resident); the CTA that completes a pair -- the one that owns it whole, or the last to
-// arrive -- reads the scores back once the pair's maximum and sum are known.  Runs without the cluster merge.
+// it is computed (4 bytes a row, L2-resident) and is read back once the pair's maximum and sum are known: by the CTA that owns the pair
+// whole, by each CTA of a cluster for its own rows, or by the CTA that arrives last.
+
+// weights[r] += exp(score[r] - M) / L for rows [lo, hi): the loads of eight rows a thread are in flight together
+template <bool kPrecise>
+__device__ __forceinline__ void add_weights(float* w, const float* scores, int lo, int hi, float M, float inv, int tid, int threads)
+{
+    for (int r0 = lo + tid; r0 < hi; r0 += 8 * threads) {
+        float s[8], x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = r0 + i * threads;
+            s[i] = r < hi ? __ldcg(scores + r) : 0.f;
+            x[i] = r < hi ? w[r] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (r0 + i * threads < hi) w[r0 + i * threads] = fmaf(kPrecise ? expf(s[i] - M) : fast_exp2(s[i] - M), inv, x[i]);
+    }
+}
+// the new token's: its weight replaces what the row's slot held
+template <bool kPrecise>
+__device__ __forceinline__ void set_new_weight(const FfaStepParams& P, int bh, int b, int row, float score, float M, float inv)
+{
+    P.weights[(size_t)bh * P.Lmax + row] = (kPrecise ? expf(score - M) : fast_exp2(score - M)) * inv;
+    if (P.positions != nullptr) P.positions[(size_t)bh * P.Lmax + row] = P.seen != nullptr ? P.seen[b] : row;
+}
+
 template <typename T, int DH, bool kWeigh>
 // Register budget: 4 resident CTAs of 160 threads (or 2 of 288) need <= 96 registers per thread;
 // head_dim 80 keeps five vectors per lane in flight and is compiled for 2 CTAs of 160 threads.
@@ -441,7 +467,7 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                 }
             }
             if constexpr (kWeigh) {
-                if (wrote_out && sr.ok) {
+                if (wrote_out && sr.ok && !cl) {
                     // the pair's maximum and sum, from this CTA's groups or from the splits' partials
                     float MM = M, LL = 0.f;
                     if (whole) {
@@ -456,12 +482,8 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                         }
                     }
                     const float inv = 1.f / LL;   // the new token was scored: the sum is at least 1 at the maximum
-                    float* w = P.weights + (size_t)bh * P.Lmax;
-                    for (int r = sr.first + ctid; r < sr.row; r += nct) w[r] += expo(__ldcg(pair_scores + r) - MM) * inv;
-                    if (ctid == 0) {
-                        w[sr.row] = expo(__ldcg(pair_scores + sr.row) - MM) * inv;
-                        if (P.positions != nullptr) P.positions[(size_t)bh * P.Lmax + sr.row] = P.seen != nullptr ? P.seen[b] : sr.row;
-                    }
+                    add_weights<kPrecise>(P.weights + (size_t)bh * P.Lmax, pair_scores, sr.first, sr.row, MM, inv, ctid, nct);
+                    if (ctid == 0) set_new_weight<kPrecise>(P, bh, b, sr.row, __ldcg(pair_scores + sr.row), MM, inv);
                 }
             }
             if (push && wrote_out) __threadfence_system();   // this thread's rows are at the peers before the pair is counted
@@ -507,6 +529,25 @@ __global__ void __launch_bounds__(DH == 80 ? 288 : 320, DH == 80 ? 1 : 2) ffa_st
                     if (d == 0) part[DH] = MM, part[DH + 1] = L;
                 }
             }
+        }
+        if constexpr (kWeigh) {   // K == 1: the pair's maximum and sum from the slots in CTA 0, the scores of this CTA's own rows
+            const int b = bh / P.H;
+            const SampleRange sr = sample_range(P, b);
+            if (sr.ok && u0 < u1) {
+                float MM = -CUDART_INF_F, LL = 0.f;
+                for (int c = 0; c < Q; ++c) MM = fmaxf(MM, ld_peer_smem_f32(clp + c * (DH + 2) + DH, 0));
+                for (int c = 0; c < Q; ++c) {
+                    const float mc = ld_peer_smem_f32(clp + c * (DH + 2) + DH, 0);
+                    if (mc != -CUDART_INF_F) LL = fmaf(kPrecise ? expf(mc - MM) : fast_exp2(mc - MM), ld_peer_smem_f32(clp + c * (DH + 2) + DH + 1, 0), LL);
+                }
+                const float inv = 1.f / LL;
+                const int j0 = (int)(u0 - (long long)bh * upb), j1 = (int)(u1 - (long long)bh * upb);
+                const float* scores = P.scores + (size_t)bh * P.score_stride;
+                add_weights<kPrecise>(P.weights + (size_t)bh * P.Lmax, scores, max(sr.first, j0 * R), min(sr.row, j1 * R), MM, inv, threadIdx.x, blockDim.x);
+                const int jt = sr.row / R;
+                if (threadIdx.x == 0 && j0 <= jt && jt < j1) set_new_weight<kPrecise>(P, bh, b, sr.row, __ldcg(scores + sr.row), MM, inv);
+            }
+            cluster_sync_all();   // CTA 0's slots have been read
         }
         if (push && leader && K == 1) {
             __threadfence_system();   // rows at the peers before the pair is counted
