@@ -20,7 +20,8 @@ namespace {
 //            and its sum into every CTA of the cluster;                                              -- cluster barrier --
 //            every CTA now has all beams' logsumexp and 128 scores that exist: the num-th largest of them is a lower bound of
 //            the num-th best score (the quarters' maxima serve when too few warps have one, as in a first step with one live beam)
-//   pass 2   (L1 / L2) every element at or above the bound goes into the leader CTA's list, about num of them; -- barrier --
+//   pass 2   (L1 / L2) the lanes whose maximum reaches the bound look at their part again; every element at or above it goes into
+//            the leader CTA's list, about num of them;                                                -- cluster barrier --
 //            the leader ranks the list and writes the result.
 // Where more elements reach the bound than the list holds (a vocabulary of ties), the cluster finds the exact border instead: a
 // radix selection, 8 bits a pass, over the 64-bit score and then the index.
@@ -103,20 +104,31 @@ __device__ __forceinline__ uint4 load_skewed(const uint4* p, unsigned skew)
 template <typename T, typename F>
 __device__ __forceinline__ void visit_segment(const T* row, int vocab, int seg, int segs, int lane, F&& f)
 {
-    constexpr int EPV = Elem<T>::EPV;
+    constexpr int EPV = Elem<T>::EPV, AT_ONCE = 4;   // vectors whose loads are in flight together
     const unsigned skew = (unsigned)(reinterpret_cast<uintptr_t>(row) & 15u);
     const int ahead = (int)(skew / sizeof(T));
-    const int vecs = (vocab + EPV - 1) / EPV;
-    for (int v = seg * 32 + lane; v < vecs; v += segs * 32) {
-        const int t0 = v * EPV;
-        float x[EPV];
-        if (t0 >= ahead && t0 - ahead + (skew != 0 ? 2 * EPV : EPV) <= vocab) {
-            Elem<T>::unpack(load_skewed(reinterpret_cast<const uint4*>(row + t0 - ahead), skew), x);
-        } else {
+    const int vecs = (vocab + EPV - 1) / EPV, step = segs * 32;
+    auto inside = [&](int t0) { return t0 >= ahead && t0 - ahead + (skew != 0 ? 2 * EPV : EPV) <= vocab; };
+    for (int v0 = seg * 32 + lane; v0 < vecs; v0 += AT_ONCE * step) {
+        uint4 raw[AT_ONCE];
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) x[e] = t0 + e < vocab ? Elem<T>::to_float(row[t0 + e]) : -CUDART_INF_F;
+        for (int i = 0; i < AT_ONCE; ++i) {
+            const int t0 = (v0 + i * step) * EPV;
+            if (v0 + i * step < vecs && inside(t0)) raw[i] = load_skewed(reinterpret_cast<const uint4*>(row + t0 - ahead), skew);
         }
-        f(x, t0);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            if (v0 + i * step >= vecs) break;
+            const int t0 = (v0 + i * step) * EPV;
+            float x[EPV];
+            if (inside(t0)) {
+                Elem<T>::unpack(raw[i], x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < EPV; ++e) x[e] = t0 + e < vocab ? Elem<T>::to_float(row[t0 + e]) : -CUDART_INF_F;
+            }
+            f(x, t0);
+        }
     }
 }
 
@@ -127,7 +139,7 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
     __shared__ __align__(16) SelRecord records[kSelSegments];
     __shared__ __align__(16) SelCandidate list[kSelList];
     __shared__ double lse[kMaxBeams];
-    __shared__ float bound_of[4 * kSelSegments];
+    __shared__ __align__(16) float bound_of[4 * kSelSegments];
     __shared__ unsigned hist[256];
     __shared__ unsigned count;
     __shared__ float s_bound;
@@ -210,18 +222,25 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
         if (lane == 0) lse[i] = (double)top + log(sum);
     }
     __syncthreads();
-    // lower bound of the num-th best score: the num-th largest of scores that exist, rounded down to fp32
-    auto find_bound = [&](int n) {
+    // lower bound of the num-th best score: the num-th largest of scores that exist, rounded down to fp32.  Each of n scores is ranked
+    // by kSelThreads / n threads, which compare it with a share of the others and add up (n is a power of two).
+    auto find_bound = [&](auto n_tag) {
+        constexpr int n = decltype(n_tag)::value, SHARE = kSelThreads / n;
         __syncthreads();
-        if (tid < n) {
-            const float me = bound_of[tid];
-            int above = 0;
-            for (int i = 0; i < n; ++i) {
-                const float x = bound_of[i];
-                above += x > me || (x == me && i < tid);
-            }
-            if (above == P.num - 1) s_bound = me;
+        const int i = tid / SHARE, part = tid % SHARE;
+        const float me = bound_of[i];
+        int above = 0;
+#pragma unroll 8
+        for (int k = part * (n / SHARE); k < (part + 1) * (n / SHARE); k += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(bound_of + k);
+            above += x.x > me || (x.x == me && k < i);
+            above += x.y > me || (x.y == me && k + 1 < i);
+            above += x.z > me || (x.z == me && k + 2 < i);
+            above += x.w > me || (x.w == me && k + 3 < i);
         }
+#pragma unroll
+        for (int off = SHARE / 2; off >= 1; off >>= 1) above += __shfl_xor_sync(0xffffffffu, above, off);
+        if (part == 0 && above == P.num - 1) s_bound = me;
         __syncthreads();
     };
     auto record_score = [&](int s, float x) -> float {
@@ -231,10 +250,10 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
         return v > -CUDART_INF ? __double2float_rd(v) : -CUDART_INF_F;   // also where v is NaN
     };
     if (tid < kSelSegments) bound_of[tid] = record_score(tid, records[tid].m);
-    find_bound(kSelSegments);
+    find_bound(std::integral_constant<int, kSelSegments>{});
     if (s_bound == -CUDART_INF_F) {
         bound_of[tid] = record_score(tid >> 2, records[tid >> 2].quarter[tid & 3]);
-        find_bound(4 * kSelSegments);
+        find_bound(std::integral_constant<int, 4 * kSelSegments>{});
     }
     const double bound = (double)s_bound;
 
@@ -250,6 +269,7 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
         // the smallest logit that can reach `least`, a little lower than it is so that rounding cannot lose one
         const double need = least - (double)s0 + base;
         const float low = __double2float_rd(need - 1e-6 * (1.0 + fabs(least) + fabs((double)s0) + fabs(base)));
+        if (m < low) return;   // this lane's largest logit, from pass 1: hardly a lane in a hundred looks at its part again
         visit_segment(row, vocab, seg, segs, lane, [&](const float (&x)[EPV], int t0) {
             float top = x[0];
 #pragma unroll
@@ -328,6 +348,7 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
         for (int i = tid; i < n; i += kSelThreads) {
             const SelCandidate c = list[i];
             int above = 0;
+#pragma unroll 4
             for (int k = 0; k < n; ++k) above += list[k].score > c.score || (list[k].score == c.score && list[k].flat < c.flat);
             if (above < P.num) {
                 const size_t o = (size_t)b * P.num + above;

@@ -126,6 +126,13 @@ Shape measured_shape(const ffa_plan* p, int row_bytes, long long rows_total, int
     if (tensors == 1) return s;   // the refinements below were measured on the exact kernel (K and V tiles)
     const double bytes = (double)rows_total * row_bytes * tensors;
     const long long BH = (long long)p->B * p->H;
+    if (p->accumulating && bytes >= 500e6) {
+        // accumulating steps pause at the end of every pair to add its weights: twice the warps do that in half the time, and a third
+        // stage keeps HBM busier meanwhile (bf16 x 128, 1024 pairs x 2047 rows: 184.5 -> 171.7 us; 256 pairs x 4000: 90.9 -> 87.7;
+        // 1024 pairs x 500, 262 MB: 50.9 against 53.7)
+        s.warps = 8, s.stages = 3;
+        return s;
+    }
     if (bytes < 48e6) {
         // every (batch, head) a CTA walks costs a serial latency chain (merge, store); with many
         // pairs and short sequences let resident CTAs overlap those chains: <= 2 pairs per CTA
@@ -699,7 +706,10 @@ int ffa_attention_accumulate(ffa_plan_t* plan, const void* q, const void* k, con
     if (weights == nullptr) return fail(FFA_ERR_ARG, "null weights");
     WeighArgs w;
     w.weights = weights, w.positions = positions, w.seen = seen;
-    return run_step(plan, q, k, v, k_cache, v_cache, out, softmax_scale, t, seq_lengths, 1, 0.f, nullptr, PageArgs{}, stream, w);
+    plan->accumulating = true;
+    const int r = run_step(plan, q, k, v, k_cache, v_cache, out, softmax_scale, t, seq_lengths, 1, 0.f, nullptr, PageArgs{}, stream, w);
+    plan->accumulating = false;
+    return r;
 }
 
 int ffa_selftest_wait_timeout(ffa_plan_t* plan, unsigned int limit_ms, void* stream)

@@ -9,6 +9,7 @@
 struct ffa_plan {
     int dtype, B, H, Dh, Lmax, use_default, device, mode;
     int prune_path;  // 0 = choose, 1 = fused cluster kernel only, 2 = streaming kernel only
+    bool accumulating;  // the call being planned is an accumulating step (ffa_attention_accumulate)
     int cluster_merge;  // 1 = merge split pairs inside a thread-block cluster when the cut allows it
     // answers of the occupancy query for cluster launches, keyed by (threads, shared memory, cluster size)
     struct { int threads, smem, cluster, clusters; } occ[8];
