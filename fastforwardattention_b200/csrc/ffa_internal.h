@@ -169,7 +169,7 @@ struct FfaBeamParams {
 };
 constexpr int kMaxBeams = 32;
 constexpr int kMaxBeamCandidates = 64;
-int ffa_k_beam_select(int dtype, const FfaBeamParams& P, cudaStream_t stream);
+int ffa_k_beam_select(int dtype, const FfaBeamParams& P, int sms, cudaStream_t stream);
 // Reordering of the caches by parent beam (ffa_cache_reorder).
 struct FfaReorderParams {
     void* k_cache;        // [groups * beams, H, Lmax, Dh]
@@ -177,6 +177,7 @@ struct FfaReorderParams {
     const int* parents;   // [groups, beams]
     int groups, beams, H, Lmax, first, rows, row_bytes;
     int chunks;           // blocks per (group, head) and tensor (set by the launcher)
+    unsigned tensors_apart;
     int* status;
 };
 int ffa_k_reorder(FfaReorderParams P, int sms, cudaStream_t stream);

@@ -59,7 +59,11 @@ int ffa_beam_select(int dtype, int batch, int beams, int vocab, long long row_st
     P.logits = logits, P.scores = scores, P.finished = finished;
     P.out_scores = out_scores, P.out_parents = out_parents, P.out_tokens = out_tokens;
     P.row_stride = row_stride, P.batch = batch, P.beams = beams, P.vocab = vocab, P.num = num, P.pad_token = pad_token;
-    const int r = ffa_k_beam_select(dtype, P, static_cast<cudaStream_t>(stream));
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return ffa_cuda_fail(e, "device query");
+    const int r = ffa_k_beam_select(dtype, P, sms, static_cast<cudaStream_t>(stream));
     if (r != 0) return ffa_cuda_fail(r, "beam selection launch");
     ffa_count_launches(1);
     return FFA_OK;
@@ -76,6 +80,7 @@ int ffa_cache_reorder(ffa_plan_t* plan, void* k_cache, void* v_cache, const int*
         return ffa_fail(FFA_ERR_RANGE, "need 0 <= first_row (%d) <= rows (%d) <= %d", first_row, rows, plan->Lmax);
     if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
     if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
+    if ((long long)plan->B * plan->H >= (1LL << 24)) return ffa_fail(FFA_ERR_RANGE, "sizes exceed int range");
     if (first_row == rows) return FFA_OK;
     FfaReorderParams P;
     std::memset(&P, 0, sizeof(P));

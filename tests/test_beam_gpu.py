@@ -35,7 +35,8 @@ def candidates(dt, B, N, V, seed=0, spread=3.0):
 
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("B,N,V,num", [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 17, 4), (1, 4, 50272, 8), (3, 5, 1001, 10), (2, 8, 50400, 16), (1, 32, 3001, 64),
-                                       (5, 7, 256, 14), (1, 1, 200003, 64), (40, 2, 333, 2)])
+                                       (5, 7, 256, 14), (1, 1, 200003, 64), (40, 2, 333, 2), (80, 3, 1200, 6), (150, 4, 700, 64), (300, 1, 901, 3),
+                                       (300, 17, 100, 20), (200, 32, 64, 64)])
 def test_select(dt, B, N, V, num):
     check(*candidates(dt, B, N, V, seed=V + num), num)
 
@@ -73,6 +74,16 @@ def test_select_ties(dt):
     check(logits, scores, 40)
     logits[1, 2, 17] = 30.0     # one candidate above a sea of equal ones
     check(logits, scores, 7)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,N,num", [(2, 8, 16), (2, 32, 64), (40, 8, 16), (160, 16, 40), (310, 4, 64)])
+def test_select_one_beam_far_ahead(dt, B, N, num):
+    """All candidates come from one beam, whose tokens lie close together."""
+    logits, scores = candidates(dt, B, N, 4000, seed=N, spread=0.5)
+    scores[torch.arange(B), torch.arange(B) % N] += 30.0
+    _, parents, _ = check(logits, scores, num)
+    assert (parents.cpu() == (torch.arange(B) % N)[:, None]).all()
 
 
 @pytest.mark.parametrize("dt", DTYPES)
