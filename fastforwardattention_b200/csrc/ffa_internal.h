@@ -177,7 +177,6 @@ struct FfaReorderParams {
     const int* parents;   // [groups, beams]
     int groups, beams, H, Lmax, first, rows, row_bytes;
     int chunks;           // blocks per (group, head) and tensor (set by the launcher)
-    unsigned tensors_apart;
     int* status;
 };
 int ffa_k_reorder(FfaReorderParams P, int sms, cudaStream_t stream);

@@ -103,8 +103,7 @@ void ffa_k_tree_shape(int dtype, int head_dim, int rows, FfaTreeShape* s)
         s->tile_us = 0.6 + 4.0 * s->tile_rows * kTreeKeys * head_dim / (2 * 128 * 0.55 * 1900);
     } else {
         const int tiles = (rows + kUmmaRows - 1) / kUmmaRows;   // of about equal height
-        s->tile_rows = (rows + tiles - 1) / tiles, s->tile_keys = kUmmaKeys;
-        s->ctas_per_sm = umma_ctas_per_sm(head_dim, umma_rep(s->tile_rows));
+        s->tile_rows = (rows + tiles - 1) / tiles, s->tile_keys = kUmmaKeys, s->ctas_per_sm = umma_ctas_per_sm(head_dim);
         // measured, one CTA to an SM: the chain S - softmax - O per tile, longer for Dh 256 by its products
         s->tile_us = head_dim > 128 ? 1.5 : umma_rep(s->tile_rows) == 1 ? 0.9 : 0.75;
     }
@@ -131,8 +130,7 @@ int ffa_k_tree_prepare(int dtype, int head_dim)
         constexpr int DH = decltype(dh)::value;
         for (int rows : {32, 64, 128}) {
             const int e = with_copies<T, DH>(rows, [&](auto kernel) {
-                return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 umma_smem(DH, umma_rep(rows)));
+                return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, umma_smem(DH));
             });
             if (e != 0) return e;
         }
@@ -165,7 +163,7 @@ int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaSt
         using T = decltype(t);
         constexpr int DH = decltype(dh)::value;
         const int r = with_copies<T, DH>(P.tile_rows, [&](auto kernel) {
-            return (int)launch_pdl(kernel, grid, kUmmaThreads, umma_smem(DH, umma_rep(P.tile_rows)), 0, true, stream, U);
+            return (int)launch_pdl(kernel, grid, kUmmaThreads, umma_smem(DH), 0, true, stream, U);
         });
         return r != 0 || P.splits == 1 ? r : merge<T, DH>(P, stream);
     });

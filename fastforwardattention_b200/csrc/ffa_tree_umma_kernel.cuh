@@ -9,8 +9,7 @@
 // padded to 128 rows (64 KB of K and V take 2.8 us of an SM's share of HBM, the products 0.5 us): what bounds a long cache is HBM.
 //
 // Warps: 0 issues the TMA loads, 1 allocates TMEM and issues the products, 2..5 do the softmax (a warp can only reach the 32 TMEM
-// lanes of its rank modulo 4).  S has two buffers, so that S of the next tile is computed while the softmax of this one runs (but see
-// umma_s_buffers).
+// lanes of its rank modulo 4).  S has two buffers, so that S of the next tile is computed while the softmax of this one runs.
 // Few query rows are copied: up to 32 rows stand in the product's 128 four times, up to 64 twice (REP), and each copy weighs its
 // share of the tile's keys, with zeros for the others -- the copies' results are added at the end.  All four warps then work on any
 // tree, and the chain of waits and instructions per tile, not a throughput, is what a softmax warp spends its time on.
@@ -39,13 +38,10 @@ constexpr int kFmaPairs = 3;       // of 8 pairs of exponentials, those that the
 constexpr int umma_dp(int dh) { return (dh + 63) / 64 * 64; }
 constexpr int umma_tile_bytes(int dh) { return umma_dp(dh) * 2 * kUmmaKeys; }
 constexpr int umma_q_bytes(int dh) { return umma_dp(dh) * 2 * kUmmaRows; }
-// Buffers of S (and P) in TMEM: with one, S of the next tile waits until O has taken P.  Dh 64 with copied rows then needs 128 columns
-// and 80 registers a thread, and four CTAs to an SM hide that and more: the tile's chain is latency, and a tile is only 16 KB.
-constexpr int umma_s_buffers(int dh, int rep) { return umma_dp(dh) == 64 && rep >= 2 ? 1 : 2; }
-constexpr int umma_ctas_per_sm(int dh, int rep) { return umma_s_buffers(dh, rep) == 1 ? 4 : umma_dp(dh) <= 128 ? 2 : 1; }
-constexpr int umma_tmem_cols(int dh, int rep) { return 512 / umma_ctas_per_sm(dh, rep); }   // Dh + 64 or 128 columns, a power of two
+constexpr int umma_ctas_per_sm(int dh) { return umma_dp(dh) <= 128 ? 2 : 1; }   // TMEM: Dh + 128 columns of 512
+constexpr int umma_tmem_cols(int dh) { return umma_dp(dh) <= 128 ? 256 : 512; }
 // ring buffers of one K or V tile each: what is left of an SM's shared memory
-constexpr int umma_stages(int dh, int rep) { return umma_s_buffers(dh, rep) == 1 ? 4 : umma_dp(dh) == 64 ? 12 : 5; }
+constexpr int umma_stages(int dh) { return umma_dp(dh) == 64 ? 12 : 5; }
 // behind Q and the ring
 struct UmmaTail {
     uint64_t bars[2 * kUmmaMaxStages + 8];
@@ -54,7 +50,7 @@ struct UmmaTail {
     int flags[1];                      // a wait ran out
     int any_bad;
 };
-constexpr int umma_smem(int dh, int rep) { return umma_q_bytes(dh) + umma_stages(dh, rep) * umma_tile_bytes(dh) + (int)sizeof(UmmaTail); }
+constexpr int umma_smem(int dh) { return umma_q_bytes(dh) + umma_stages(dh) * umma_tile_bytes(dh) + (int)sizeof(UmmaTail); }
 
 struct FfaTreeUmmaParams {
     CUtensorMap q, k_new, v_new, k_cache, v_cache;
@@ -249,10 +245,9 @@ __device__ __forceinline__ float2 exp2_fma(float2 y)
 }
 
 template <typename T, int DH, int REP>
-__global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_tree_umma_kernel(const __grid_constant__ FfaTreeUmmaParams U)
+__global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_umma_kernel(const __grid_constant__ FfaTreeUmmaParams U)
 {
-    constexpr int DP = umma_dp(DH), NB = DP / 64, TILE = umma_tile_bytes(DH), STAGES = umma_stages(DH, REP), ROWB = DH * 2;
-    constexpr int SB = umma_s_buffers(DH, REP);
+    constexpr int DP = umma_dp(DH), NB = DP / 64, TILE = umma_tile_bytes(DH), STAGES = umma_stages(DH), ROWB = DH * 2;
     constexpr int BOX = 64 * 128;   // bytes of a tile's box: 64 rows of 128 bytes
     constexpr uint32_t S_COL = DP;  // TMEM columns: O at 0, the two S / P buffers behind it
     constexpr int QUADS = 4 / REP, COLS = kUmmaKeys / REP;   // warps per copy of the query rows; keys of a tile that a copy weighs
@@ -297,7 +292,7 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // after pdl_wait: a CTA that held TMEM while it waits for the previous grid could keep that grid from ever finishing
-    if (warp == 1) tmem_alloc(smem_u32(&tail.tmem_base), umma_tmem_cols(DH, REP)), tmem_relinquish();
+    if (warp == 1) tmem_alloc(smem_u32(&tail.tmem_base), umma_tmem_cols(DH)), tmem_relinquish();
     tcgen05_before_sync();
     __syncthreads();
     tcgen05_after_sync();
@@ -315,7 +310,7 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
                         tma_load_2d(q_smem + x * (kUmmaRows * 128) + (i * QUADS + w) * (kQBoxRows * 128), &U.q, 64 * x,
                                     cut.bh * R + row0 + w * kQBoxRows, q_full);
             uint32_t stage = 0, use = 0;
-            // loads in the order the products take them: K0, K1, V0, K2, V1, ..., V(last); with one buffer of S K0, V0, K1, V1, ...
+            // loads in the order the products take them: K0, K1, V0, K2, V1, ..., V(last)
             auto load = [&](int j, bool is_v) -> bool {
                 const int u = cut.u0 + j;
                 if (use > 0 && !mbar_wait_bounded(empty + 8 * stage, (use - 1) & 1, dead)) return false;
@@ -335,13 +330,9 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
                 if (++stage == STAGES) stage = 0, ++use;
                 return true;
             };
-            if constexpr (SB == 2) {
-                bool ok = load(0, false);
-                for (int j = 1; ok && j < n_tiles; ++j) ok = load(j, false) && load(j - 1, true);
-                if (ok) load(n_tiles - 1, true);
-            } else {
-                for (int j = 0; j < n_tiles && load(j, false) && load(j, true); ++j) {}
-            }
+            bool ok = load(0, false);
+            for (int j = 1; ok && j < n_tiles; ++j) ok = load(j, false) && load(j - 1, true);
+            if (ok) load(n_tiles - 1, true);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -356,11 +347,11 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
             if (++stage == STAGES) stage = 0, phase ^= 1;
         };
         auto values = [&](int j) -> bool {   // O += P_j V_j
-            if (!together(mbar_wait_bounded(p_ready + 8 * (j % SB), (j / SB) & 1, dead))) return false;
+            if (!together(mbar_wait_bounded(p_ready + 8 * (j & 1), (j >> 1) & 1, dead))) return false;
             if (!together(mbar_wait_bounded(full + 8 * stage, phase, dead))) return false;
             tcgen05_after_sync();
             const uint64_t v = v_desc + stage * (TILE / 16);
-            const uint32_t p = tmem + S_COL + kUmmaKeys * (j % SB);
+            const uint32_t p = tmem + S_COL + kUmmaKeys * (j & 1);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < kUmmaKeys / 16; ++k)   // 16 keys: 8 columns of packed P, two atoms of V
@@ -374,26 +365,25 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
         };
         bool ok = together(mbar_wait_bounded(q_full, 0, dead));
         for (int j = 0; ok && j < n_tiles; ++j) {
-            // S_j goes where P_(j-2) was, or P_(j-1) with one buffer: that product has to be through
+            // S_j goes where P_(j-2) was: that product has to be through
             ok = together(mbar_wait_bounded(full + 8 * stage, phase, dead) &&
-                          (j < SB || mbar_wait_bounded(pv_done + 8 * ((j - SB) & 1), ((j - SB) >> 1) & 1, dead)));
+                          (j < 2 || mbar_wait_bounded(pv_done + 8 * (j & 1), ((j >> 1) - 1) & 1, dead)));
             if (!ok) break;
             tcgen05_after_sync();
             const uint64_t k = k_desc + stage * (TILE / 16);
-            const uint32_t s = tmem + S_COL + kUmmaKeys * (j % SB);
+            const uint32_t s = tmem + S_COL + kUmmaKeys * (j & 1);
             if (elect_one()) {
 #pragma unroll
                 for (int x = 0; x < DP / 16; ++x)
                     umma_ss(s, q_desc + ((x / 4) * (kUmmaRows * 128) + (x % 4) * 32) / 16, k + ((x / 4) * BOX + (x % 4) * 32) / 16, S_DESC, x > 0);
                 umma_commit(empty + 8 * stage);
-                umma_commit(s_full + 8 * (j % SB));
+                umma_commit(s_full + 8 * (j & 1));
             }
             __syncwarp();
             next();
-            if (SB == 1) ok = values(j);
-            else if (j > 0) ok = values(j - 1);
+            if (j > 0) ok = values(j - 1);
         }
-        if (SB == 2 && ok) values(n_tiles - 1);
+        if (ok) values(n_tiles - 1);
         // products in flight end before their operands and TMEM go away, also when a wait ran out
         if (elect_one()) {
             umma_commit(drained);
@@ -440,10 +430,10 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
                 uint4 new0, new1;
                 if (sent < news) new0 = fetch(sent);
                 if (sent + threads < news) new1 = fetch(sent + threads);
-                ok = together(mbar_wait_bounded(s_full + 8 * (j % SB), (j / SB) & 1, dead));
+                ok = together(mbar_wait_bounded(s_full + 8 * (j & 1), (j >> 1) & 1, dead));
                 if (!ok) break;
                 tcgen05_after_sync();
-                const uint32_t s_addr = lanes + S_COL + kUmmaKeys * (j % SB);
+                const uint32_t s_addr = lanes + S_COL + kUmmaKeys * (j & 1);
                 uint32_t s[COLS];
                 if constexpr (COLS == 64) tmem_ld32<0>(s_addr, s), tmem_ld32<32>(s_addr + 32, s);
                 else if constexpr (COLS == 32) tmem_ld32<0>(s_addr + 32 * rep, s);
@@ -536,7 +526,7 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
                 if (masked) {
                     // What V holds outside the valid rows, and infinities and NaN of drafted tokens, must not meet a weight of 0:
                     // cleared in shared memory (the latter remembered for the end).
-                    const uint32_t at = SB == 1 ? 2 * j + 1 : j < n_tiles - 1 ? 2 * j + 2 : 2 * n_tiles - 1;   // V_j's place in the order of loads
+                    const uint32_t at = j < n_tiles - 1 ? 2 * j + 2 : 2 * n_tiles - 1;   // V_j's place in the order of loads
                     const uint32_t slot = at % STAGES;
                     ok = together(mbar_wait_bounded(full + 8 * slot, (at / STAGES) & 1, dead));
                     if (!ok) break;
@@ -561,7 +551,7 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
                 }
                 tmem_wait_st();
                 tcgen05_before_sync();
-                mbar_arrive(p_ready + 8 * (j % SB));
+                mbar_arrive(p_ready + 8 * (j & 1));
                 if (sent < news) append(sent, new0);
                 if (sent + threads < news) append(sent + threads, new1);
                 sent += 2 * threads;
@@ -654,7 +644,7 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH, REP)) ffa_t
     tcgen05_before_sync();
     __syncthreads();
     tcgen05_after_sync();
-    if (warp == 1) tmem_dealloc(tmem, umma_tmem_cols(DH, REP));
+    if (warp == 1) tmem_dealloc(tmem, umma_tmem_cols(DH));
     if (tid == 0 && flags[0]) {
         atomicOr(P.status, kStatusWaitTimeout);
         // a wait ran out: let the copies already issued land before the CTA releases its shared memory (bounded again)
