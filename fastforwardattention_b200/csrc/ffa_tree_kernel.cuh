@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(256) ffa_tree_accept_kernel(const FfaAcceptPar
     const int vpr = P.row_bytes / 16;
     const int* path = P.path + (size_t)b * P.path_len;
     const int n = P.seq_lengths != nullptr ? P.seq_lengths[b] : P.t;
-    if (n < 0 || n >= P.Lmax) {
+    if (n < 0 || n > P.Lmax) {   // (a full cache has an empty path)
         if (threadIdx.x == 0) atomicOr(P.status, kStatusBadLength);
         return;
     }

@@ -263,7 +263,6 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
                    pv_done = p_ready + 16, drained = pv_done + 16;
     volatile int* dead = flags;
 
-    pdl_release();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int R = P.groups * P.tokens;
     if (tid == 0) {
@@ -291,11 +290,13 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // after pdl_wait: a CTA that held TMEM while it waits for the previous grid could keep that grid from ever finishing
+    // TMEM after pdl_wait: a CTA that held some while it waits for the previous grid could keep that grid from ever finishing; and
+    // the next grid may start only when this one has its own
     if (warp == 1) tmem_alloc(smem_u32(&tail.tmem_base), umma_tmem_cols(DH)), tmem_relinquish();
     tcgen05_before_sync();
     __syncthreads();
     tcgen05_after_sync();
+    pdl_release();
     const uint32_t tmem = tail.tmem_base;
     const int n_tiles = cut.u1 - cut.u0;
     uint32_t issued = 0;   // K and V loads of the issuing thread

@@ -410,7 +410,14 @@ struct FastForwardAttn {
         torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({B, H, Dh}, k_cache.options());
         TORCH_CHECK(out.is_cuda() && out.device() == device && dtype_code(out) == dtype && out.is_contiguous() && out.numel() == n,
                     "FastForwardAttn: out must be a contiguous tensor of batch*heads*head_dim elements on the engine's device");
-        if (!has_scores) bind_workspace(true);   // once, as for pruned steps
+        if (!has_scores) {   // once, as for pruned steps
+            cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+            cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing);
+            TORCH_CHECK(capturing == cudaStreamCaptureStatusNone,
+                        "FastForwardAttn: make the first accumulating step outside of a graph capture: it binds the score scratch");
+            retired.push_back(workspace);   // graphs recorded before go on using it
+            bind_workspace(true);
+        }
         check(ffa_attention_accumulate(plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
                                        (float)softmax_scale, (int)(max_row < 0 ? Lmax - 1 : max_row), rows.data_ptr<int>(),
                                        weights.data_ptr<float>(), positions.data_ptr<int>(), seen.data_ptr<int>(),
@@ -584,6 +591,7 @@ struct FastForwardAttn {
 
     ffa_plan_t* plan = nullptr;
     torch::Tensor k_cache, v_cache, workspace, kept_mask, push_tensor;
+    std::vector<torch::Tensor> retired;   // workspaces that recorded graphs may hold
     c10::Device device{c10::kCUDA, 0};
     int64_t B = 0, H = 0, Dh = 0, Lmax = 0;
     int dtype = 0, mode = FFA_MODE_EXACT, prune_path = 0;

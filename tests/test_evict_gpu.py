@@ -78,7 +78,8 @@ def test_step_agrees_with_the_decode_step(dt):
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("D", [64, 80, 128, 256])
 @pytest.mark.parametrize("n,keep,recent,first", [(2, 1, 0, 0), (33, 32, 0, 0), (33, 32, 32, 0), (64, 32, 8, 4), (65, 64, 10, 0), (100, 37, 12, 5), (1000, 333, 100, 0),
-                                                 (1000, 999, 250, 4), (1256, 1, 1, 0), (4100, 2048, 512, 4), (20000, 5001, 1, 3)])
+                                                 (1000, 999, 250, 4), (1256, 1, 1, 0), (4100, 2048, 512, 4), (20000, 5001, 1, 3), (49152, 49151, 5, 1),
+                                                 (49153, 49152, 5, 1), (49153, 49100, 0, 0)])
 def test_evict(dt, D, n, keep, recent, first):
     ffa, kc, vc, w, pos, g = engine(dt, 2, 3, D, n + 2, seed=n + keep)
     # positions as an earlier eviction leaves them: distinct, in any order, with gaps
@@ -225,6 +226,30 @@ def test_captured_steps_and_evictions():
         assert torch.equal(out, other) and torch.equal(kept, want) and torch.equal(w, wt) and torch.equal(pos, pt)
         assert torch.equal(kc, kt) and torch.equal(vc, vt)
     assert ffa.device_status() == 0
+
+
+def test_the_first_accumulating_step_is_not_captured_and_keeps_recorded_graphs_alive():
+    dt, B, H, D, n = torch.float16, 1, 4, 64, 3000
+    ffa, kc, vc, w, pos, g = engine(dt, B, H, D, n + 2, seed=19)
+    q, k, v = (torch.randn(B, H, 1, D, generator=g, device="cuda").to(dt) for _ in range(3))
+    rows = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    want = ffa.attention_per_sample(q, k, v, 0.1, rows)
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ffa.attention_per_sample(q, k, v, 0.1, rows, out=out)
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        with pytest.raises(RuntimeError, match="outside of a graph capture"):
+            ffa.attention_accumulate(q, k, v, 0.1, rows, w, pos, rows)
+        ffa.attention_per_sample(q, k, v, 0.1, rows, out=out)
+    ffa.attention_accumulate(q, k, v, 0.1, rows, w, pos, rows)   # binds a larger workspace
+    filler = [torch.full((1 << 20,), 7, dtype=torch.int32, device="cuda") for _ in range(8)]   # takes freed memory, if there is any
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    assert ffa.device_status() == 0 and len(filler) == 8
 
 
 def test_refusals_from_python():

@@ -273,10 +273,11 @@ def test_refusals_from_python():
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-def test_paged_sequences_draft_and_accept(dt):
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_paged_sequences_draft_and_accept(dt, D):
     from fastforwardattention_b200 import PagedFastForwardAttn, PagePool
 
-    B, H, D, T = 3, 2, 128, 24
+    B, H, T = 3, 2, 24
     lens = [130, 250, 1]
     pool = PagePool(16, H, D, dt, "cuda", page_rows=128)
     pool.k.fill_(float("nan")), pool.v.fill_(float("nan"))
@@ -331,3 +332,56 @@ def test_drafting_agrees_with_one_token_steps(dt):
         assert ((step.double() - out[:, :, j].double()).abs() <= 2 * bound[:, :, j]).all()
     for x, y in zip(a.get_cache(), c.get_cache()):
         assert torch.equal(x[:, :, : n + len(path)], y[:, :, : n + len(path)])
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_offsets_beyond_32_bits(dt):
+    """Caches of more than 2^31 elements (2^33 bytes in fp32): the last pair's rows, attended, appended and moved."""
+    from fastforwardattention_b200 import FastForwardAttn
+
+    B, H, L, D, T = 8, 32, 66000, 128, 6
+    kc, vc = (torch.empty(B, H, L, D, dtype=dt, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(43)
+    n = L - T
+    for c in (kc, vc):
+        c.zero_()
+        c[-1, -1, -3000:] = torch.randn(3000, D, generator=g).to(dt).cuda()
+        c[-1, -1, : n - 2000] = torch.randn(1, D, generator=g).to(dt).cuda()
+    q, k, v = (torch.randn(B, H, T, D, generator=g).to(dt).cuda() for _ in range(3))
+    tree = random_tree(T, g).cuda()
+    ffa = FastForwardAttn.adopt(kc, vc)
+    last = lambda x: x[-1:, -1:]
+    want, bound = D64.tree_attention(last(q), last(k), last(v), last(kc), last(vc), tree, D ** -0.5, [n])
+    out = ffa.tree_attention(q, k, v, tree, D ** -0.5, n)
+    D64.assert_within(last(out), want, bound)
+    assert torch.equal(last(kc)[:, :, n:], last(k)) and torch.equal(last(vc)[:, :, n:], last(v))
+    ffa.tree_accept(torch.tensor([[1, 3, 5]] * B, dtype=torch.int32, device="cuda"), n)
+    assert torch.equal(kc[-1, -1, n: n + 3], k[-1, -1, [1, 3, 5]])
+    before = vc[-1, -1, 65000:].clone()
+    ffa.reorder(torch.tensor([[0, 1, 2, 3, 4, 5, 7, 6]], dtype=torch.int32, device="cuda"), L, first_row=65000)
+    assert torch.equal(vc[-2, -1, 65000:], before) and ffa.device_status() == 0
+
+
+def test_a_full_cache_accepts_an_empty_path():
+    dt, B, D = torch.bfloat16, 2, 64
+    ffa, kc, vc, q, k, v, tree = setup(dt, B, 1, 1, D, 20, 4, L=24, seed=47)
+    kb = kc.clone()
+    ffa.tree_accept_per_sample(torch.tensor([[-1, -1], [0, 3]], dtype=torch.int32, device="cuda"), torch.tensor([24, 20], dtype=torch.int32, device="cuda"))
+    assert ffa.device_status() == 0 and torch.equal(kc[0], kb[0]) and torch.equal(kc[1, :, 21], kb[1, :, 23])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_two_engines_on_two_streams(dt):
+    """Calls that run at the same time on engines of their own."""
+    D, T, n = 128, 30, 3000
+    cases = [setup(dt, 1, 2, 1, D, n, T, seed=50 + i) for i in range(2)]
+    want = [c[0].tree_attention(*c[3:7], D ** -0.5, n) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(c[0].tree_attention(*c[3:7], D ** -0.5, n))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
