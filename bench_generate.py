@@ -1,6 +1,6 @@
 """Whole-generation benchmark in the shape of the reference's summarize.py (summarize.py:29-145).
 
-    python bench_generate.py [--model opt-1.3b|gpt-j-6b] [--prompt 1000] [--output-len 256] [--samples 20]
+    python bench_generate.py [--model opt-1.3b|gpt-j-6b] [--prompt 1000] [--output-len 256] [--samples 20] [--beams 1]
 
 The reference times `model.generate` of a HuggingFace OPT / GPT-J over cnn_dailymail articles for
 batch sizes 1, 2, 5, 10 with three attention implementations (summarize.py:82-96: HuggingFace's own,
@@ -17,6 +17,10 @@ sides, summed over samples/batch generations, as the reference does.  Three impl
   engine         one FastForwardAttn per layer built from the prompt's K/V, one attention call per
                  layer per token -- how the reference's fork drives FFA (modeling_opt.py:201-226)
   engine-graph   the same engines, all layers of a token recorded once in a CUDA graph (GraphedLayers)
+
+With --beams N > 1 the generations are beam searches (the best N of every sample's beams and vocabulary per token): torch takes the
+log-softmax, its top N and index_selects every layer's K and V; engine uses beam_select and reorder on the engines' caches, whose
+prompt rows the beams of a sample share.
 
 Absolute seconds are not comparable with README.md:51-65 (random weights, no tokenizer, another GPU);
 the ratios between the rows are the result.  Prints one JSON line.
@@ -137,6 +141,54 @@ def generate(model, ids, new_tokens, impl):
     return torch.stack(out, 1)
 
 
+def generate_beams(model, ids, new_tokens, impl, beams):
+    """Beam search for new_tokens steps; the best sequence of every sample and its score."""
+    from fastforwardattention_b200 import FastForwardAttn, beam_select
+
+    B, T = ids.shape
+    E, V = model.cfg["width"], model.cfg["vocab"]
+    h, kvs = model.prefill(ids)
+    spread = lambda a: a.repeat_interleave(beams, 0)
+    if impl == "torch":
+        Ks, Vs = [spread(k) for k, _ in kvs], [spread(v) for _, v in kvs]
+    else:
+        engines = [FastForwardAttn(spread(k), spread(v), T + new_tokens, False) for k, v in kvs]
+    del kvs
+    scores = torch.full((B, beams), float("-inf"), device=ids.device)
+    scores[:, 0] = 0.0   # the beams of a sample start from the same prompt: one of them is enough
+    h, first_beam = spread(h), torch.arange(B, device=ids.device)[:, None] * beams
+    sequences = torch.empty(B, beams, 0, dtype=torch.int64, device=ids.device)
+    for s in range(new_tokens):
+        logits = (F.layer_norm(h, (E,)) @ model.tok.t()).view(B, beams, V)
+        if impl == "torch":
+            total = scores[..., None] + F.log_softmax(logits.float(), -1)
+            scores, at = total.view(B, beams * V).topk(beams)
+            parents, tokens = at // V, at % V
+        else:
+            scores, parents, tokens = beam_select(logits, scores, beams)
+        sequences = torch.cat([sequences.gather(1, parents.long()[..., None].expand(-1, -1, s)), tokens.long()[..., None]], -1)
+        if s == new_tokens - 1:
+            break
+        if impl == "torch":
+            rows = (first_beam + parents).flatten()
+            Ks, Vs = [k.index_select(0, rows) for k in Ks], [v.index_select(0, rows) for v in Vs]
+        else:
+            for e in engines:
+                e.reorder(parents, T + s, first_row=T)
+        x = (model.tok[tokens.flatten().long()] + model.pos[T + s + 2])[:, None]
+        for i, L in enumerate(model.layers):
+            q, k, v = model.qkv(L, x)
+            if impl == "torch":
+                Ks[i], Vs[i] = torch.cat([Ks[i], k], 2), torch.cat([Vs[i], v], 2)
+                a = torch.matmul(torch.softmax(torch.matmul(q, Ks[i].transpose(-1, -2)), dim=-1), Vs[i]).transpose(1, 2)
+            else:
+                a = engines[i].attention(q, k, v, 1.0, T + s, 0.0)
+            x = x + a.reshape(B * beams, 1, E) @ L["out"]
+            x = model.mlp(L, x)
+        h = x[:, 0]
+    return sequences[:, 0]
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--model", default="opt-1.3b", choices=sorted(MODELS))
@@ -144,11 +196,16 @@ def main():
     ap.add_argument("--output-len", type=int, default=256)   # README.md:48
     ap.add_argument("--samples", type=int, default=20, help="articles per batch size (the reference's --max_ite)")
     ap.add_argument("--batch-sizes", default="1,2,5,10")     # summarize.py:82
+    ap.add_argument("--beams", type=int, default=1, help="beams per sample; 1 = greedy decoding")
     args = ap.parse_args()
     dev = torch.device("cuda", 0)
     torch.backends.cuda.matmul.allow_fp16_reduced_precision_reduction = False
     model = Decoder(MODELS[args.model], torch.float16, dev)
-    impls = ["torch", "engine", "engine-graph"]
+    impls = ["torch", "engine", "engine-graph"] if args.beams == 1 else ["torch", "engine"]
+
+    def run(ids, new_tokens, impl):
+        return generate(model, ids, new_tokens, impl) if args.beams == 1 else generate_beams(model, ids, new_tokens, impl, args.beams)
+
     rows, agree = {i: {} for i in impls}, {}
     with torch.no_grad():
         for bs in [int(x) for x in args.batch_sizes.split(",")]:
@@ -157,12 +214,12 @@ def main():
             batches = [torch.randint(4, model.cfg["vocab"], (bs, args.prompt), generator=g, device=dev) for _ in range(n_gen)]
             tokens = {}
             for impl in impls:
-                generate(model, batches[0], 8, impl)   # warm-up: library handles, kernel attributes
+                run(batches[0], 8, impl)   # warm-up: library handles, kernel attributes
                 total = 0.0
                 for ids in batches:
                     torch.cuda.synchronize()
                     t0 = time.perf_counter()
-                    toks = generate(model, ids, args.output_len, impl)
+                    toks = run(ids, args.output_len, impl)
                     torch.cuda.synchronize()
                     total += time.perf_counter() - t0
                 tokens[impl] = toks
@@ -170,9 +227,9 @@ def main():
             # greedy choices of the last generation: identical prefix length (random weights give near-ties,
             # after the first differing token the continuations are different sequences)
             same = [int(((tokens["torch"] == tokens[i]).int().cumprod(1).sum(1).float().mean()).item()) for i in impls[1:]]
-            agree[bs] = {"engine": same[0], "engine-graph": same[1], "of": args.output_len}
+            agree[bs] = {**dict(zip(impls[1:], same)), "of": args.output_len}
     line = {"benchmark": "generate", "model_shape": args.model, "dtype": "f16", "weights": "seeded random", "prompt_tokens": args.prompt,
-            "new_tokens": args.output_len, "samples_per_batch_size": args.samples, "unit": "seconds summed over samples/batch generations",
+            "new_tokens": args.output_len, "beams": args.beams, "samples_per_batch_size": args.samples, "unit": "seconds summed over samples/batch generations",
             "seconds": rows, "speedup_vs_torch": {i: {bs: round(rows["torch"][bs] / rows[i][bs], 2) for bs in rows[i]} for i in impls[1:]},
             "tokens_identical_to_torch_up_to": agree}
     print(json.dumps(line))
