@@ -78,8 +78,8 @@ def lib() -> C.CDLL:
         L.ffa_peer_gather.argtypes = [vp, vp, vp, i, C.c_uint, vp]
         L.ffa_peer_push_target.argtypes = [vp, vp]
         L.ffa_tree_scratch_bytes.argtypes = [vp, i, i, i, C.POINTER(sz)]
-        L.ffa_tree_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, vp, f, i, vp, i, vp, i, i, vp, sz, vp]
-        L.ffa_tree_accept.argtypes = [vp, vp, vp, vp, i, i, vp, vp, i, i, vp]
+        L.ffa_tree_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, i, vp, f, i, vp, i, vp, i, i, i, vp, sz, vp]
+        L.ffa_tree_accept.argtypes = [vp, vp, vp, vp, i, i, vp, vp, i, i, i, vp]
         L.ffa_attention_accumulate.argtypes = [vp, vp, vp, vp, vp, vp, vp, f, i, vp, vp, vp, vp, vp]
         L.ffa_evict.argtypes = [vp, vp, vp, vp, vp, vp, i, i, i, i, vp, vp]
         L.ffa_beam_select.argtypes = [i, i, i, i, C.c_longlong, vp, vp, vp, i, i, vp, vp, vp, vp]

@@ -114,7 +114,7 @@ struct FfaTreeParams {
     float* partials;             // [B*H][row_tiles][splits][part_rows][Dh + 4]; null when splits == 1
     int* status;
     const int* page_table;       // as in FfaStepParams
-    int max_pages, page_rows;
+    int max_pages, page_rows, pool_pages;
 };
 // Floats of a partial result's row: the weighted sum, its maximum, its sum of exponentials, and two to keep rows 16-byte aligned
 constexpr int ffa_tree_part_stride(int head_dim) { return head_dim + 4; }
@@ -127,7 +127,7 @@ struct FfaAcceptParams {
     int path_len, B, H, Lmax, t, row_bytes;
     int* status;
     const int* page_table;
-    int max_pages, page_rows;
+    int max_pages, page_rows, pool_pages;
 };
 // How a tree attention is cut: query rows per CTA, tiles of them, rows of a partial result, keys per tile, and what the choice of the
 // number of splits needs to know of the kernel that takes this type and number of query rows: resident CTAs per SM, and the time that

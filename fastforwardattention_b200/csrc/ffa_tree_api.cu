@@ -1,6 +1,7 @@
 // C entries of the tree attention (include/ffa_c_api.h): argument checks, the cut over CTAs and the parameter fill.
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstring>
 
 #include "../../include/ffa_c_api.h"
@@ -55,9 +56,11 @@ int check_sizes(const ffa_plan* plan, int groups, int tokens, int t)
     return FFA_OK;
 }
 
-int check_pages(const ffa_plan* plan, const int* page_table, int max_pages, int page_rows)
+int check_pages(const ffa_plan* plan, const int* page_table, int max_pages, int page_rows, int pool_pages)
 {
     if (page_table == nullptr) return FFA_OK;
+    if (pool_pages <= 0 || (long long)pool_pages * plan->H * (page_rows > 0 ? page_rows : 1) >= (1LL << 31))
+        return ffa_fail(FFA_ERR_RANGE, "pool_pages = %d: must be positive, and the pool's rows below 2^31", pool_pages);
     if (page_rows <= 0 || page_rows % 128 != 0)
         return ffa_fail(FFA_ERR_RANGE, "page_rows (%d) must be a positive multiple of 128", page_rows);
     if (max_pages <= 0 || (long long)max_pages * page_rows != plan->Lmax)
@@ -80,7 +83,7 @@ int ffa_tree_scratch_bytes(const ffa_plan_t* plan, int groups, int tokens, int t
 
 int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
                        const unsigned char* tree, int tree_per_sample, int groups, int tokens, void* out, float softmax_scale, int t,
-                       const int* seq_lengths, int right_or_no_padding, const int* page_table, int max_pages, int page_rows,
+                       const int* seq_lengths, int right_or_no_padding, const int* page_table, int max_pages, int page_rows, int pool_pages,
                        void* scratch, size_t scratch_bytes, void* stream)
 {
     int r = check_sizes(plan, groups, tokens, t);
@@ -88,11 +91,12 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
     if (!q || !k || !v || !k_cache || !v_cache || !tree || !out) return ffa_fail(FFA_ERR_ARG, "null tensor pointer");
     if (!ffa_aligned16(q) || !ffa_aligned16(k) || !ffa_aligned16(v) || !ffa_aligned16(k_cache) || !ffa_aligned16(v_cache) || !ffa_aligned16(out))
         return ffa_fail(FFA_ERR_ARG, "tensor pointers must be 16-byte aligned");
+    if (!std::isfinite(softmax_scale)) return ffa_fail(FFA_ERR_RANGE, "softmax_scale is not finite");
     if (seq_lengths == nullptr && !right_or_no_padding)
         return ffa_fail(FFA_ERR_ARG, "left padding (right_or_no_padding = 0) needs seq_lengths");
     if ((seq_lengths == nullptr || !right_or_no_padding) && tokens > plan->Lmax - t)
         return ffa_fail(FFA_ERR_RANGE, "t + tokens (%d + %d) exceeds the cache length %d", t, tokens, plan->Lmax);
-    r = check_pages(plan, page_table, max_pages, page_rows);
+    r = check_pages(plan, page_table, max_pages, page_rows, pool_pages);
     if (r != FFA_OK) return r;
     if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
     if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
@@ -111,7 +115,7 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
     P.scale = softmax_scale;
     P.splits = s.splits, P.row_tiles = s.row_tiles, P.part_rows = s.part_rows, P.tile_rows = s.tile_rows;
     P.partials = static_cast<float*>(scratch), P.status = plan->status;
-    P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows;
+    P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows, P.pool_pages = pool_pages;
     r = ffa_k_tree_attention(plan->dtype, plan->Dh, P, static_cast<cudaStream_t>(stream));
     if (r != 0) return ffa_cuda_fail(r, "tree attention launch");
     ffa_count_launches(s.splits > 1 ? 2 : 1);
@@ -119,14 +123,14 @@ int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const voi
 }
 
 int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* path, int path_len, int t, const int* seq_lengths,
-                    const int* page_table, int max_pages, int page_rows, void* stream)
+                    const int* page_table, int max_pages, int page_rows, int pool_pages, void* stream)
 {
     if (plan == nullptr) return ffa_fail(FFA_ERR_ARG, "null plan");
     if (path_len < 0 || path_len > kTreeMaxRows) return ffa_fail(FFA_ERR_RANGE, "path length %d outside [0, %d]", path_len, kTreeMaxRows);
     if (t < 0 || t >= plan->Lmax) return ffa_fail(FFA_ERR_RANGE, "t = %d outside [0, %d)", t, plan->Lmax);
     if (!k_cache || !v_cache || (path_len > 0 && !path)) return ffa_fail(FFA_ERR_ARG, "null tensor pointer");
     if (!ffa_aligned16(k_cache) || !ffa_aligned16(v_cache)) return ffa_fail(FFA_ERR_ARG, "tensor pointers must be 16-byte aligned");
-    int r = check_pages(plan, page_table, max_pages, page_rows);
+    int r = check_pages(plan, page_table, max_pages, page_rows, pool_pages);
     if (r != FFA_OK) return r;
     if (plan->offline) return ffa_fail(FFA_ERR_ARG, "this plan was created offline (planning only) and cannot launch");
     if (plan->ws == nullptr) return ffa_fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
@@ -136,7 +140,7 @@ int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* p
     P.k_cache = k_cache, P.v_cache = v_cache, P.path = path, P.seq_lengths = seq_lengths, P.path_len = path_len;
     P.B = plan->B, P.H = plan->H, P.Lmax = plan->Lmax, P.t = t, P.row_bytes = plan->Dh * ffa_elem_size(plan->dtype);
     P.status = plan->status;
-    P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows;
+    P.page_table = page_table, P.max_pages = max_pages, P.page_rows = page_rows, P.pool_pages = pool_pages;
     r = ffa_k_tree_accept(P, static_cast<cudaStream_t>(stream));
     if (r != 0) return ffa_cuda_fail(r, "tree accept launch");
     ffa_count_launches(1);

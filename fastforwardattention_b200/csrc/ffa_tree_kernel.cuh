@@ -40,6 +40,20 @@ struct TreeCut {
     __device__ __forceinline__ bool owns_new_tokens() const { return split == splits - 1 && rt == 0; }
 };
 
+// Whether a page that the sample's rows 0..row+tokens-1 need is missing from its table; the same for all threads of the CTA.
+__device__ __forceinline__ bool tree_page_missing(const FfaTreeParams& P, int b, const SampleRange& sr)
+{
+    bool missing = false;
+    if (P.page_table != nullptr && sr.ok) {
+        const int pages = (sr.row + P.tokens + P.page_rows - 1) / P.page_rows;
+        for (int i = threadIdx.x; i < pages; i += blockDim.x) {
+            const int page = P.page_table[(size_t)b * P.max_pages + i];
+            missing = missing || page < 0 || page >= P.pool_pages;
+        }
+    }
+    return P.page_table != nullptr && __syncthreads_or(missing);
+}
+
 // k and v of the drafted tokens -> rows n..n+tokens-1 of the cache: vectors first, first + step, ... of the tokens' 16-byte vectors
 __device__ __forceinline__ void tree_append(const FfaTreeParams& P, int bh, int row, int rowb, int first, int step)
 {
@@ -166,8 +180,9 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
     const bool whole = P.splits == 1;
     float* out = static_cast<float*>(P.out) + ((size_t)cut.bh * R + row0) * DH;
     float* part = whole ? nullptr : tree_partial(P, cut.bh, cut.rt, cut.split, DH);
-    if (!cut.sr.ok && tid == 0) atomicOr(P.status, kStatusBadLength);   // refused: zeros, nothing appended
-    if (!cut.sr.ok || cut.split >= cut.splits) {
+    const bool missing = tree_page_missing(P, cut.b, cut.sr);
+    if ((!cut.sr.ok || missing) && tid == 0) atomicOr(P.status, missing ? kStatusBadIndex : kStatusBadLength);   // refused: zeros, nothing appended
+    if (!cut.sr.ok || missing || cut.split >= cut.splits) {
         if (!whole) tree_empty_partial(part, rows, DH, tid, kTreeThreads);
         else for (int i = tid; i < rows * DH; i += kTreeThreads) out[i] = 0.f;
         return;
@@ -342,7 +357,12 @@ __global__ void __launch_bounds__(256) ffa_tree_accept_kernel(const FfaAcceptPar
     for (; count < P.path_len; ++count) {
         const int j = path[count];
         if (j < 0) break;
-        if (j <= prev || j >= P.Lmax - n) {
+        bool missing = false;
+        if (P.page_table != nullptr && j >= 0 && j < P.Lmax - n) {   // the row itself and the one it moves to
+            const int from = P.page_table[(size_t)b * P.max_pages + (n + j) / P.page_rows], to = P.page_table[(size_t)b * P.max_pages + (n + count) / P.page_rows];
+            missing = from < 0 || from >= P.pool_pages || to < 0 || to >= P.pool_pages;
+        }
+        if (j <= prev || j >= P.Lmax - n || missing) {
             if (threadIdx.x == 0) atomicOr(P.status, kStatusBadIndex);
             return;
         }

@@ -151,8 +151,7 @@ int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaSt
     FfaTreeUmmaParams U;
     U.p = P;
     const long long pairs = (long long)P.B * P.H;
-    // a pool's number of pages is not known here: its bound is only there to be larger than every row
-    const long long cache_rows = P.page_table != nullptr ? 0x7fffffffLL : pairs * P.Lmax;
+    const long long cache_rows = P.page_table != nullptr ? (long long)P.pool_pages * P.H * P.page_rows : pairs * P.Lmax;
     int e = encode(&U.q, dtype, P.q, head_dim, pairs * rows, kQBoxRows);
     if (e == 0) e = encode(&U.k_new, dtype, P.k, head_dim, pairs * P.tokens, kUmmaKeys);
     if (e == 0) e = encode(&U.v_new, dtype, P.v, head_dim, pairs * P.tokens, kUmmaKeys);

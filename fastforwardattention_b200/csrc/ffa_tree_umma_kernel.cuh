@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
     const bool whole = P.splits == 1;
     T* out = static_cast<T*>(P.out) + ((size_t)cut.bh * R + row0) * DH;
     float* part = whole ? nullptr : tree_partial(P, cut.bh, cut.rt, cut.split, DH);
-    if (!cut.sr.ok && tid == 0) atomicOr(P.status, kStatusBadLength);   // refused: zeros, nothing appended
-    if (!cut.sr.ok || cut.split >= cut.splits) {
+    const bool missing = tree_page_missing(P, cut.b, cut.sr);
+    if ((!cut.sr.ok || missing) && tid == 0) atomicOr(P.status, missing ? kStatusBadIndex : kStatusBadLength);   // refused: zeros, nothing appended
+    if (!cut.sr.ok || missing || cut.split >= cut.splits) {
         if (!whole) tree_empty_partial(part, rows, DH, tid, kUmmaThreads);
         else for (int i = tid; i < rows * DH; i += kUmmaThreads) Elem<T>::store(out + i, 0.f);
         return;

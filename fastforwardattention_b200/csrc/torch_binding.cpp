@@ -47,6 +47,7 @@ struct TreeTarget {
     torch::Tensor k, v;              // caches or page pools
     const torch::Tensor* table;      // [B, max_pages] or null
     int64_t max_pages, page_rows;
+    int pool_pages() const { return table ? (int)k.size(0) : 0; }
     const int* table_ptr() const { return table ? table->data_ptr<int>() : nullptr; }
 };
 
@@ -98,7 +99,7 @@ torch::Tensor run_tree(const TreeTarget& T, const torch::Tensor& q_, const torch
     check(ffa_tree_attention(T.plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), T.k.data_ptr(), T.v.data_ptr(),
                              static_cast<const unsigned char*>(tree.data_ptr()), tree.dim() == 3, (int)groups, (int)n, out.data_ptr(),
                              (float)softmax_scale, (int)t, rows_ ? rows.data_ptr<int>() : nullptr, !left_padding, T.table_ptr(),
-                             (int)T.max_pages, (int)T.page_rows, bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                             (int)T.max_pages, (int)T.page_rows, T.pool_pages(), bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
                              at::cuda::getCurrentCUDAStream().stream()),
           "tree attention");
     return out;
@@ -115,7 +116,7 @@ void run_accept(const TreeTarget& T, const torch::Tensor& path_, int64_t t, cons
     c10::cuda::CUDAGuard guard(T.device);
     torch::Tensor k = T.k, v = T.v;
     check(ffa_tree_accept(T.plan, k.data_ptr(), v.data_ptr(), path.numel() > 0 ? path.data_ptr<int>() : nullptr, (int)path.size(1), (int)t,
-                          rows_ ? rows.data_ptr<int>() : nullptr, T.table_ptr(), (int)T.max_pages, (int)T.page_rows,
+                          rows_ ? rows.data_ptr<int>() : nullptr, T.table_ptr(), (int)T.max_pages, (int)T.page_rows, T.pool_pages(),
                           at::cuda::getCurrentCUDAStream().stream()),
           "tree accept");
 }

@@ -184,20 +184,22 @@ int ffa_attention_paged(ffa_plan_t* plan, const void* q, const void* k, const vo
  * the bound t or has no room for its tokens is refused: FFA_STATUS_BAD_LENGTH, output zero, nothing appended).
  * A query row that sees nothing is 0.  A token that a row does not see has no influence on it, whatever its values.
  * Statistics and sums are fp32; fp16 and bf16 weights are rounded to the tensors' type before they meet V, and the result once.
- * groups * tokens <= 1024.  page_table: NULL, or the paged caches of ffa_attention_paged.
+ * groups * tokens <= 1024.  page_table: NULL, or the paged caches of ffa_attention_paged with pools of pool_pages pages; every page
+ * that holds rows 0..row+tokens-1 of a sequence has to be in its table (a sequence with an entry outside [0, pool_pages) there is
+ * refused: FFA_STATUS_BAD_INDEX, output zero, nothing appended).
  * scratch: ffa_tree_scratch_bytes(plan, groups, tokens, t) bytes of device memory (may be 0), 16-byte aligned, used by this call
  * only. */
 int ffa_tree_scratch_bytes(const ffa_plan_t* plan, int groups, int tokens, int t, size_t* bytes);
 int ffa_tree_attention(ffa_plan_t* plan, const void* q, const void* k, const void* v, void* k_cache, void* v_cache,
                        const unsigned char* tree, int tree_per_sample, int groups, int tokens, void* out, float softmax_scale,
                        int t, const int* seq_lengths, int right_or_no_padding, const int* page_table, int max_pages,
-                       int page_rows, void* scratch, size_t scratch_bytes, void* stream);
+                       int page_rows, int pool_pages, void* scratch, size_t scratch_bytes, void* stream);
 /* Keeps the accepted path of a tree: rows row + path[b, i] -> row + i of both caches, in place, i = 0, 1, ... up to the first
  * negative entry.  path [batch, path_len] (device): strictly increasing tree indices (a node's ancestors come before it), so that no row is
- * overwritten before it has moved; row = t, or seq_lengths[b].  A sample whose path is not increasing or leaves the cache is
- * left as it was (FFA_STATUS_BAD_INDEX). */
+ * overwritten before it has moved; row = t, or seq_lengths[b].  A sample whose path is not increasing, leaves the cache or names a
+ * row without a page is left as it was (FFA_STATUS_BAD_INDEX). */
 int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* path, int path_len, int t, const int* seq_lengths,
-                    const int* page_table, int max_pages, int page_rows, void* stream);
+                    const int* page_table, int max_pages, int page_rows, int pool_pages, void* stream);
 
 /* ---- A cache held at a budget of rows: eviction by accumulated attention weight.  No counterpart in the reference.
  * ffa_attention_accumulate is one exact decode step (ffa_attention with p = 0; always fp32 arithmetic, whatever the plan's mode)

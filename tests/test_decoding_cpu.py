@@ -21,7 +21,7 @@ def plan():
 
 def tree_args(p, **kw):
     a = dict(plan=p, q=P16, k=P16, v=P16, kc=P16, vc=P16, tree=P16, per_sample=0, groups=1, tokens=8, out=P16, scale=1.0, t=100, lengths=None,
-             right=1, table=None, max_pages=0, page_rows=0, scratch=None, bytes=0, stream=None)
+             right=1, table=None, max_pages=0, page_rows=0, pool=64, scratch=None, bytes=0, stream=None)
     a.update(kw)
     return list(a.values())
 
@@ -31,6 +31,8 @@ def tree_args(p, **kw):
     (dict(groups=0), RANGE), (dict(tokens=0), RANGE), (dict(tokens=-3), RANGE), (dict(groups=3, tokens=400), RANGE), (dict(tokens=1 << 30, groups=4), RANGE),
     (dict(t=-1), RANGE), (dict(t=4096), RANGE), (dict(t=4089), RANGE), (dict(right=0), ARG),
     (dict(table=P16, max_pages=4, page_rows=100), RANGE), (dict(table=P16, max_pages=4, page_rows=128), RANGE),
+    (dict(table=P16, max_pages=32, page_rows=128, pool=0), RANGE), (dict(table=P16, max_pages=32, page_rows=128, pool=1 << 30), RANGE),
+    (dict(scale=float("nan")), RANGE), (dict(scale=float("inf")), RANGE),
     (dict(), ARG)])   # the last one is in order, but this plan cannot launch
 def test_tree_attention_refusals(plan, kw, code):
     L, p = plan
@@ -41,7 +43,7 @@ def test_tree_attention_refusals(plan, kw, code):
                                      (dict(n=1025), RANGE), (dict(t=4096), RANGE), (dict(), ARG)])
 def test_tree_accept_refusals(plan, kw, code):
     L, p = plan
-    a = dict(plan=p, kc=P16, vc=P16, path=P16, n=4, t=100, lengths=None, table=None, max_pages=0, page_rows=0, stream=None)
+    a = dict(plan=p, kc=P16, vc=P16, path=P16, n=4, t=100, lengths=None, table=None, max_pages=0, page_rows=0, pool=64, stream=None)
     a.update(kw)
     assert L.ffa_tree_accept(*a.values()) == code, L.ffa_last_error()
 

@@ -68,7 +68,14 @@ def test_step_agrees_with_the_decode_step(dt):
         q, k, v = (torch.randn(B, H, 1, D, generator=g, device="cuda").to(dt) for _ in range(3))
         sl = torch.full((B,), n, dtype=torch.int32, device="cuda")
         w.zero_()
+        ffa.set_cluster_merge(False)   # the splits' partials through global memory, the last arriver adds all weights
+        through_global = ffa.attention_accumulate(q, k, v, D ** -0.5, sl, w, pos, sl, max_row=n)
+        wg = w.clone()
+        ffa.set_cluster_merge(True)
+        w.zero_()
         out = ffa.attention_accumulate(q, k, v, D ** -0.5, sl, w, pos, sl, max_row=n)
+        _, bound, _, pb = D64.step_weights(q, k, v, kc, vc, D ** -0.5, [n] * B)
+        assert ((out.double() - through_global.double()).abs() <= 2 * bound).all() and ((w.double() - wg.double()).abs() <= 2 * pb).all()
         ref = ffa.attention(q, k, v, D ** -0.5, n, 0)
         _, bound, _, pb = D64.step_weights(q, k, v, kc, vc, D ** -0.5, [n] * B)
         assert ((out.double() - ref.double()).abs() <= 2 * bound).all()   # each within its bound of the exact value

@@ -385,3 +385,37 @@ def test_two_engines_on_two_streams(dt):
                 got.append(c[0].tree_attention(*c[3:7], D ** -0.5, n))
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_pages_that_are_missing_or_outside_the_pool_are_refused(dt):
+    """Every sequence stands on its own: those whose rows have no page are reported and left, the others go on."""
+    from fastforwardattention_b200 import PagePool, _extension
+
+    B, H, D, T, pr = 5, 2, 64, 20, 128
+    pool = PagePool(12, H, D, dt, "cuda", page_rows=pr)
+    pool.k.normal_(), pool.v.normal_()
+    engine = _extension().PagedEngine(pool.k, pool.v, B, 4)
+    rows = [120, 120, 250, 130, 10]
+    table = torch.tensor([[0, 1, -1, -1], [2, -1, -1, -1], [3, 12, 4, -1], [-1, 5, 6, -1], [7, -1, -1, -1]], dtype=torch.int32)
+    q, k, v = (torch.randn(B, H, T, D, device="cuda").to(dt) for _ in range(3))
+    tree = torch.ones(T, T, dtype=torch.bool, device="cuda").tril()
+    sl = torch.tensor(rows, dtype=torch.int32, device="cuda")
+    kb, vb = pool.k.clone(), pool.v.clone()
+    out = engine.tree_attention_per_sample(q, k, v, tree, table.cuda(), D ** -0.5, sl)
+    assert engine.device_status() == 4 and (out[1:4] == 0).all()
+    flat = lambda p, pages: torch.cat([p[i] for i in pages], 1)[None]
+    for b, pages in ((0, [0, 1]), (4, [7])):
+        one = slice(b, b + 1)
+        want, bound = D64.tree_attention(q[one], k[one], v[one], flat(kb, pages), flat(vb, pages), tree, D ** -0.5, [rows[b]])
+        D64.assert_within(out[one], want, bound)
+        assert torch.equal(flat(pool.k, pages)[0, :, rows[b]: rows[b] + T], k[b])
+    assert torch.equal(pool.k[[2, 3, 4, 5, 6, 8, 9, 10, 11]], kb[[2, 3, 4, 5, 6, 8, 9, 10, 11]])
+    kb = pool.k.clone()
+    path = torch.tensor([[0, 19], [0, 19], [1, 2], [3, 4], [118, 119]], dtype=torch.int32, device="cuda")
+    engine.tree_accept_per_sample(path, table.cuda(), sl)
+    assert engine.device_status() == 4
+    # sequences 1 (row 139), 2 (row 251) and 4 (row 128) name rows of missing pages; of sequence 3 only the first page is missing, and its
+    # rows 133, 134 -> 130, 131 lie in the second one (page 5, rows 5, 6 -> 2, 3)
+    kb[5, :, 2:4] = kb[5, :, 5:7].clone()
+    assert torch.equal(pool.k[0, :, 121], kb[1, :, 11]) and torch.equal(pool.k[2:], kb[2:])
