@@ -160,8 +160,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) ffa_tree_merge_kernel(const 
 //   P   through shared memory, transposed, the groups of rows XORed with the key so that neither side has bank conflicts
 //   O   a thread keeps RT rows x DH / 16 columns
 // K and V have one buffer each: V of a tile arrives while S is computed, K of the next one while O is.  Rows outside the valid range
-// are zero-filled, never read, so that what a cache holds behind its last row cannot reach the result.  What bounds it: HBM for a few rows,
-// fp32 FMAs from about 16 on.
+// are zero-filled, never read, so that what a cache holds behind its last row cannot reach the result.  What bounds it: fp32 FMAs and the
+// reads from shared memory that feed them.
 template <int DH, int RT>
 __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTreeParams P)
 {
@@ -337,6 +337,257 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
     // the drafted tokens go to the cache behind the last read of this CTA, a share from each of the pair's CTAs
     const int ctas = cut.splits * P.row_tiles, mine = cut.split * P.row_tiles + cut.rt;
     tree_append(P, cut.bh, cut.sr.row, DH * 4, mine * kTreeThreads + tid, ctas * kTreeThreads);
+}
+
+// The same for few query rows (RG * 8 of them; fp32).  With 16 x 16 threads every warp would read the whole tile from shared memory for
+// two rows of its own; here a warp owns 16 keys of a tile, for all rows: what a warp loads only it reads, so the loop has no CTA
+// barrier, and K and V pass through shared memory once.
+//   S   lane = (one of 4 groups of keys, one of 8 slices of the columns): 8 rows x 4 keys a pass, 32 products to 12 reads of 16 bytes,
+//       then added over the slices so that a lane is left with one row.  (With whole columns and 2 rows x 2 keys to a lane, 4 products
+//       to 4 reads, the kernel waits for shared memory.)
+//   O   lane = columns: all rows x DH / 32 columns, the weights broadcast from shared memory (Dh 64: half a warp each takes every other key)
+// Each warp has its own running maximum and sum; the warps meet once, at the end.  Bound by HBM while there are many pairs and at most
+// 8 rows, then by latency and shared memory.  This kernel and the one above, each at its number of splits: 256 pairs x 2000 tokens x
+// 128, 6 drafted 100 / 178 us (floor 81), 16 drafted 175 / 350; 16 pairs x 8000 x 80, 5 drafted 31 / 41; 32 pairs x 995 x 64, 5 drafted and
+// accepted 14.9 / 15.0, 12 drafted 17.3 / 17.0.
+constexpr int kFewWarps = 4, kFewKeys = 16;   // keys a warp and tile
+constexpr int few_kv_floats(int dh) { return 2 * kFewKeys * dh; }   // K and V of a warp
+constexpr int few_stages(int dh) { return dh <= 64 ? 2 : 1; }   // as many as leave room for three CTAs to an SM (by registers two, with 16 rows)
+constexpr int few_smem(int dh, int rg)
+{
+    const int ring = kFewWarps * (few_stages(dh) * few_kv_floats(dh) + kFewKeys * 8 * rg), merge = kFewWarps * 8 * rg * ffa_tree_part_stride(dh);
+    return 4 * (8 * rg * dh + (ring > merge ? ring : merge));
+}
+template <int DH, int RG>
+__global__ void __launch_bounds__(32 * kFewWarps, RG == 1 ? 3 : 2) ffa_tree_few_kernel(const FfaTreeParams P)
+{
+    constexpr int ROWS = 8 * RG, VPR = DH / 4, XV = (VPR + 31) / 32, KEYS_AT_ONCE = VPR <= 16 ? 2 : 1, KV = few_kv_floats(DH), STAGES = few_stages(DH), STRIDE = ffa_tree_part_stride(DH);
+    extern __shared__ __align__(128) unsigned char smem[];
+    float* qs = reinterpret_cast<float*>(smem);     // [ROWS][DH], scaled
+    float* area = qs + ROWS * DH;                 // K and V, then weights; at the end the warps' results
+
+    pdl_release();
+    pdl_wait();
+    const TreeCut<kTreeKeys> cut(P);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rows = P.groups * P.tokens;   // all of the pair's
+    const bool whole = P.splits == 1;
+    float* out = static_cast<float*>(P.out) + (size_t)cut.bh * rows * DH;
+    float* part = whole ? nullptr : tree_partial(P, cut.bh, 0, cut.split, DH);
+    const bool missing = tree_page_missing(P, cut.b, cut.sr);
+    if ((!cut.sr.ok || missing) && tid == 0) atomicOr(P.status, missing ? kStatusBadIndex : kStatusBadLength);   // refused: zeros, nothing appended
+    if (!cut.sr.ok || missing || cut.split >= cut.splits) {
+        if (!whole) tree_empty_partial(part, rows, DH, tid, 32 * kFewWarps);
+        else for (int i = tid; i < rows * DH; i += 32 * kFewWarps) out[i] = 0.f;
+        return;
+    }
+
+    float* ring = area + warp * STAGES * KV;                                // K, V of every stage
+    float* ps = area + kFewWarps * STAGES * KV + warp * kFewKeys * ROWS;   // [key][row]
+    // this warp's 16 keys of tile u; those outside the valid range are zero-filled, never read
+    auto load = [&](int u, bool is_v, int stage) {
+        const bool cached = u < cut.cache_tiles;
+        const int base = (cached ? cut.c0 + u : u - cut.cache_tiles) * kTreeKeys + warp * kFewKeys;
+        const int lo = cached ? cut.sr.first : 0, hi = cached ? cut.sr.row : P.tokens;
+        if (u < cut.u1 && base + kFewKeys > lo && base < hi) {
+            const size_t off = cached ? cache_row_offset(P, cut.bh, base, DH * 4) : ((size_t)cut.bh * P.tokens + base) * (DH * 4);
+            const unsigned char* src = static_cast<const unsigned char*>(is_v ? (cached ? P.v_cache : P.v) : (cached ? P.k_cache : P.k)) + off;
+            const uint32_t dst = smem_u32(ring + stage * KV + (is_v ? kFewKeys * DH : 0));
+#pragma unroll
+            for (int i0 = 0; i0 < kFewKeys * VPR; i0 += 32) {
+                const int i = i0 + lane, r = i / VPR;
+                const bool in = base + r >= lo && base + r < hi;
+                cp_async_16_or_zero(dst + i * 16, in ? src + (size_t)i * 16 : static_cast<const unsigned char*>(P.k), in ? 16u : 0u);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) load(cut.u0 + i, false, i), load(cut.u0 + i, true, i);
+    {
+        const float* q = static_cast<const float*>(P.q) + (size_t)cut.bh * rows * DH;
+        for (int i = tid; i < ROWS * DH; i += 32 * kFewWarps) qs[i] = i < rows * DH ? q[i] * P.scale : 0.f;
+    }
+    __syncthreads();
+
+    const int kg = lane >> 3, ds = lane & 7;   // this lane's keys are kg, kg + 4, ..., its chunks of 4 columns ds, ds + 8, ..., its rows ds, ds + 8
+    float m[RG], l[RG];
+    float4 o[ROWS][XV];
+#pragma unroll
+    for (int i = 0; i < RG; ++i) m[i] = -CUDART_INF_F, l[i] = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int x = 0; x < XV; ++x) o[r][x] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+    for (int u = cut.u0, stage = 0; u < cut.u1; ++u, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+        const float* ks = ring + stage * KV;
+        const float* vs = ks + kFewKeys * DH;
+        cp_async_wait<2 * STAGES - 1>();   // K is here, V and later tiles may be on their way
+        __syncwarp();
+        const bool cached = u < cut.cache_tiles;
+        const int base = (cached ? cut.c0 + u : u - cut.cache_tiles) * kTreeKeys + warp * kFewKeys;
+        const int lo = cached ? cut.sr.first : 0, hi = cached ? cut.sr.row : P.tokens;
+        const bool any = base + kFewKeys > lo && base < hi;   // some of the warp's keys are valid
+        if (any) {
+            float sum[RG][4];   // of this lane's rows and keys
+#pragma unroll
+            for (int h = 0; h < RG; ++h) {
+                float2 acc[8][4];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[r][j] = make_float2(0.f, 0.f);
+#pragma unroll (RG == 1 ? 1 : 2)   // (registers)
+                for (int i = 0; i < (VPR + 7) / 8; ++i) {
+                    const int c = ds + 8 * i;
+                    if (VPR % 8 != 0 && c >= VPR) break;
+                    float4 k4[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) k4[j] = *reinterpret_cast<const float4*>(ks + (kg + 4 * j) * DH + 4 * c);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const float4 q4 = *reinterpret_cast<const float4*>(qs + (8 * h + r) * DH + 4 * c);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            acc[r][j] = __ffma2_rn(make_float2(q4.x, q4.y), make_float2(k4[j].x, k4[j].y), acc[r][j]);
+                            acc[r][j] = __ffma2_rn(make_float2(q4.z, q4.w), make_float2(k4[j].z, k4[j].w), acc[r][j]);
+                        }
+                    }
+                }
+                // over the 8 lanes of a key: each step halves the rows that a lane holds, until its own is left
+                float a[8][4];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) a[r][j] = acc[r][j].x + acc[r][j].y;
+#pragma unroll
+                for (int n = 4; n >= 1; n >>= 1)
+#pragma unroll
+                    for (int r = 0; r < n; ++r)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const bool upper = (ds & n) != 0;
+                            const float other = __shfl_xor_sync(0xffffffffu, upper ? a[r][j] : a[r + n][j], n);
+                            a[r][j] = (upper ? a[r + n][j] : a[r][j]) + other;
+                        }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[h][j] = a[0][j];
+            }
+            __syncwarp();
+            load(u + STAGES, false, stage);
+            float corr[RG];
+            bool moved = false;
+#pragma unroll
+            for (int h = 0; h < RG; ++h) {
+                const int r = 8 * h + ds;
+                float top = m[h];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int key = base + kg + 4 * j;
+                    bool see = r < rows && key >= lo && key < hi;
+                    if (!cached && see) see = P.tree[((size_t)(P.tree_per_sample ? cut.b : 0) * P.tokens + r % P.tokens) * P.tokens + key] != 0;
+                    if (!see) sum[h][j] = -CUDART_INF_F;
+                    top = fmaxf(top, sum[h][j]);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));   // over the row's lanes
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                const float ref = top == -CUDART_INF_F ? 0.f : top;   // nothing seen so far: every weight is 0, not NaN
+                corr[h] = expf(m[h] - ref);
+                moved = moved || top != m[h];
+                m[h] = top;
+                float w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ps[(kg + 4 * j) * ROWS + r] = w[j] = expf(sum[h][j] - ref);
+                l[h] = fmaf(l[h], corr[h], (w[0] + w[1]) + (w[2] + w[3]));   // this lane's keys; the lanes are added at the end
+            }
+            cp_async_wait<2 * STAGES - 1>();   // V is here
+            __syncwarp();
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int r = 0; r < ROWS; ++r) {
+                    const float f = __shfl_sync(0xffffffffu, corr[r >> 3], r & 7);
+#pragma unroll
+                    for (int x = 0; x < XV; ++x) o[r][x].x *= f, o[r][x].y *= f, o[r][x].z *= f, o[r][x].w *= f;
+                }
+            }
+            auto values = [&](auto guard_tag) {
+                constexpr bool kGuard = decltype(guard_tag)::value;
+#pragma unroll
+                for (int k0 = 0; k0 < kFewKeys; k0 += KEYS_AT_ONCE) {
+                    const int k = KEYS_AT_ONCE == 2 ? k0 + (lane >> 4) : k0;
+#pragma unroll
+                    for (int x = 0; x < XV; ++x) {
+                        const int c = (KEYS_AT_ONCE == 2 ? lane & 15 : lane) + 32 * x;
+                        if (c >= VPR) break;
+                        const float4 v4 = *reinterpret_cast<const float4*>(vs + k * DH + 4 * c);
+#pragma unroll
+                        for (int r0 = 0; r0 < ROWS; r0 += 4) {
+                            const float4 p4 = *reinterpret_cast<const float4*>(ps + k * ROWS + r0);
+                            const float pr[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (kGuard && pr[i] == 0.f) continue;   // a hidden token has no part in the row, whatever its values
+                                const float2 pp = make_float2(pr[i], pr[i]);
+                                const float2 a = __ffma2_rn(pp, make_float2(v4.x, v4.y), make_float2(o[r0 + i][x].x, o[r0 + i][x].y));
+                                const float2 b = __ffma2_rn(pp, make_float2(v4.z, v4.w), make_float2(o[r0 + i][x].z, o[r0 + i][x].w));
+                                o[r0 + i][x] = make_float4(a.x, a.y, b.x, b.y);
+                            }
+                        }
+                    }
+                }
+            };
+            if (cached) values(std::false_type{});
+            else values(std::true_type{});
+        }
+        __syncwarp();   // V and the weights may be overwritten
+        if (!any) load(u + STAGES, false, stage);
+        load(u + STAGES, true, stage);
+    }
+    cp_async_wait<0>();
+
+    // the warps' results: [warp][row][columns, maximum, sum]
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < RG; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8), l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+        float* to = area + (size_t)(warp * ROWS + 8 * h + ds) * STRIDE;
+        if (kg == 0) to[DH] = m[h], to[DH + 1] = l[h];
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int x = 0; x < XV; ++x) {
+            if (KEYS_AT_ONCE == 2) {   // the half-warps' keys
+                o[r][x].x += __shfl_xor_sync(0xffffffffu, o[r][x].x, 16), o[r][x].y += __shfl_xor_sync(0xffffffffu, o[r][x].y, 16);
+                o[r][x].z += __shfl_xor_sync(0xffffffffu, o[r][x].z, 16), o[r][x].w += __shfl_xor_sync(0xffffffffu, o[r][x].w, 16);
+            }
+            const int c = lane + 32 * x;
+            if (c >= VPR) break;
+            *reinterpret_cast<float4*>(area + (size_t)(warp * ROWS + r) * STRIDE + 4 * c) = o[r][x];
+        }
+    __syncthreads();
+    for (int i = tid; i < rows * VPR; i += 32 * kFewWarps) {
+        const int r = i / VPR, c = i - r * VPR;
+        float M = -CUDART_INF_F, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) M = fmaxf(M, area[(size_t)(w * ROWS + r) * STRIDE + DH]);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) {
+            const float* from = area + (size_t)(w * ROWS + r) * STRIDE;
+            const float f = from[DH] == -CUDART_INF_F && from[DH + 1] == 0.f ? 0.f : expf(from[DH] - M);   // 0: saw nothing
+            const float4 y = *reinterpret_cast<const float4*>(from + 4 * c);
+            L = fmaf(f, from[DH + 1], L);
+            sum.x = isfinite(y.x) ? fmaf(f, y.x, sum.x) : sum.x + y.x, sum.y = isfinite(y.y) ? fmaf(f, y.y, sum.y) : sum.y + y.y;
+            sum.z = isfinite(y.z) ? fmaf(f, y.z, sum.z) : sum.z + y.z, sum.w = isfinite(y.w) ? fmaf(f, y.w, sum.w) : sum.w + y.w;
+        }
+        const float inv = whole ? (L == 0.f ? 0.f : 1.f / L) : 1.f;
+        float* to = whole ? out + (size_t)r * DH : part + (size_t)r * STRIDE;
+        *reinterpret_cast<float4*>(to + 4 * c) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        if (!whole && c == 0) to[DH] = M, to[DH + 1] = L;
+    }
+    tree_append(P, cut.bh, cut.sr.row, DH * 4, cut.split * 32 * kFewWarps + tid, cut.splits * 32 * kFewWarps);
 }
 
 // Rows n + path[i] -> n + i of every pair, in place.  A thread owns one 16-byte column of K or V and walks the path: indices

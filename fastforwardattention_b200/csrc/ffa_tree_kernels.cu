@@ -10,20 +10,24 @@ using namespace ffa_dev;
 
 namespace {
 
-// query rows per thread of the CUDA-core kernel (16 threads deep): as few as hold all rows, at most four
+// fp32: the kernel whose warps own keys takes up to 16 query rows (its buffers and results would not fit at head_dim 256), the one
+// whose threads own rows the others, with as few rows per thread (16 threads deep) as hold all, at most four
+bool simt_few(int head_dim, int rows) { return head_dim <= 128 && rows <= 16; }
 int simt_rt(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 template <int DH, typename F>
 int with_rows(int rows, F&& f)
 {
-    switch (simt_rt(rows)) {
-        case 1: return f(ffa_tree_simt_kernel<DH, 1>);
-        case 2: return f(ffa_tree_simt_kernel<DH, 2>);
-        default: return f(ffa_tree_simt_kernel<DH, 4>);
+    if constexpr (DH <= 128) {
+        if (simt_few(DH, rows)) return rows <= 8 ? f(ffa_tree_few_kernel<DH, 1>) : f(ffa_tree_few_kernel<DH, 2>);
+    } else if (simt_rt(rows) == 1) {
+        return f(ffa_tree_simt_kernel<DH, 1>);
     }
+    return simt_rt(rows) <= 2 ? f(ffa_tree_simt_kernel<DH, 2>) : f(ffa_tree_simt_kernel<DH, 4>);
 }
 constexpr int kSmemPerSm = 228 * 1024;
 int simt_smem(int head_dim, int rows)
 {
+    if (simt_few(head_dim, rows)) return few_smem(head_dim, rows <= 8 ? 1 : 2);
     const int bm = 16 * simt_rt(rows);
     return 4 * (bm * head_dim + kTreeKeys * (head_dim + 4) + kTreeKeys * head_dim + kTreeKeys * bm);
 }
@@ -96,11 +100,14 @@ int merge(const FfaTreeParams& P, cudaStream_t stream)
 void ffa_k_tree_shape(int dtype, int head_dim, int rows, FfaTreeShape* s)
 {
     if (dtype == 0) {
-        s->tile_rows = 16 * simt_rt(rows), s->tile_keys = kTreeKeys;
+        const bool few = simt_few(head_dim, rows);
+        s->tile_rows = few ? (rows <= 8 ? 8 : 16) : 16 * simt_rt(rows), s->tile_keys = kTreeKeys;
         const int fit = kSmemPerSm / (simt_smem(head_dim, rows) + 1024);
-        s->ctas_per_sm = fit > 4 ? 4 : fit;
-        // S and O of a tile: 4 * rows * keys * Dh flops at about 55 % of an SM's 128 FMAs a cycle, and two memory latencies
-        s->tile_us = 0.6 + 4.0 * s->tile_rows * kTreeKeys * head_dim / (2 * 128 * 0.55 * 1900);
+        const int most = few ? (rows <= 8 ? 3 : 2) : 4;   // by registers
+        s->ctas_per_sm = fit > most ? most : fit;
+        // S and O of a tile: 4 * rows * keys * Dh flops at about 55 % of an SM's 128 FMAs a cycle (30 % with a warp a scheduler), and two
+        // memory latencies
+        s->tile_us = 0.6 + 4.0 * s->tile_rows * kTreeKeys * head_dim / (2 * 128 * (few ? 0.3 : 0.55) * 1900);
     } else {
         const int tiles = (rows + kUmmaRows - 1) / kUmmaRows;   // of about equal height
         s->tile_rows = (rows + tiles - 1) / tiles, s->tile_keys = kUmmaKeys, s->ctas_per_sm = umma_ctas_per_sm(head_dim);
@@ -116,7 +123,7 @@ int ffa_k_tree_prepare(int dtype, int head_dim)
     if (dtype == 0)
         return dispatch32(head_dim, [&](auto dh) -> int {
             constexpr int DH = decltype(dh)::value;
-            for (int rows : {16, 32, 64}) {
+            for (int rows : {8, 16, 32, 64}) {
                 const int e = with_rows<DH>(rows, [&](auto kernel) {
                     return (int)cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, simt_smem(DH, rows));
                 });
@@ -145,7 +152,7 @@ int ffa_k_tree_attention(int dtype, int head_dim, const FfaTreeParams& P, cudaSt
     if (dtype == 0)
         return dispatch32(head_dim, [&](auto dh) -> int {
             constexpr int DH = decltype(dh)::value;
-            const int e = with_rows<DH>(rows, [&](auto kernel) { return (int)launch_pdl(kernel, grid, kTreeThreads, simt_smem(DH, rows), 0, true, stream, P); });
+            const int e = with_rows<DH>(rows, [&](auto kernel) { return (int)launch_pdl(kernel, grid, simt_few(DH, rows) ? 32 * kFewWarps : kTreeThreads, simt_smem(DH, rows), 0, true, stream, P); });
             return e != 0 || P.splits == 1 ? e : merge<float, DH>(P, stream);
         });
     FfaTreeUmmaParams U;

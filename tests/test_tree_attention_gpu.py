@@ -88,6 +88,34 @@ def test_left_padding(dt):
     assert ffa.device_status() == 0
 
 
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("G,T", [(1, 8), (3, 3), (1, 15), (2, 8), (1, 17)])
+def test_few_query_rows_in_fp32(D, G, T):
+    """Row counts around those where the fp32 kernels take turns; lengths and padding that leave warps without keys; a row that sees nothing
+    but the cache, and at length 0 nothing at all; with several CTAs to a pair and with few."""
+    n, some = 1500, [0, 5, 41, 1499, 1500, 1497, 64, 1425]
+    for B in (4, 64):
+        at = (some * B)[:B]
+        dev = torch.tensor(at, dtype=torch.int32, device="cuda")
+        for padded in (False, True):
+            ffa, kc, vc, q, k, v, tree = setup(torch.float32, B, 4, G, D, n, T, seed=D + T)
+            lo, hi = (at, [n] * B) if padded else ([0] * B, at)
+            for b in range(B):   # what is outside the valid rows never matters
+                for c in (kc, vc):
+                    c[b, :, :lo[b]], c[b, :, hi[b]:] = float("nan"), float("inf")
+            tree[..., T - 1, :] = False
+            want, bound = D64.tree_attention(q, k, v, kc.clone(), vc.clone(), tree, D ** -0.5, hi, lo)
+            if padded:
+                out = ffa.tree_attention(q, k, v, tree, D ** -0.5, n, seq_lengths=dev)
+            else:
+                out = ffa.tree_attention_per_sample(q, k, v, tree, D ** -0.5, dev, max_row=n)
+                assert (out[0].view(4, G, T, D)[:, :, T - 1] == 0).all()
+            D64.assert_within(out, want, bound, f"{B} sequences, padded {padded}")
+            for b in range(B):
+                assert torch.equal(kc[b, :, hi[b]:hi[b] + T], k[b]) and torch.equal(vc[b, :, hi[b]:hi[b] + T], v[b])
+            assert ffa.device_status() == 0
+
+
 @pytest.mark.parametrize("dt", DTYPES)
 @pytest.mark.parametrize("n,T", [(0, 6), (130, 6), (130, 70), (4000, 20)])
 def test_hidden_and_stale_values_have_no_influence(dt, n, T):
