@@ -169,6 +169,7 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
     __shared__ __align__(16) SelCandidate list[kSelList];
     __shared__ double lse[kMaxBeams];
     __shared__ __align__(16) uint32_t bound_of[4 * kSelSegments];
+    __shared__ __align__(16) uint32_t lane_best[kSelThreads];
     __shared__ uint2 found[kSelShare];          // elements of this CTA that may reach the bound: index, logit
     __shared__ float beam_score[kMaxBeams];
     __shared__ unsigned hist[256];
@@ -264,14 +265,14 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
     __syncthreads();
     // Lower bound of the num-th best score: the num-th largest of scores that exist.  Scores are rounded down to fp32, and as integers in
     // the order of the floats their lowest bits give way to their index: all are different, and a rank is one comparison each.
-    auto find_bound = [&](int n) {
+    auto find_bound = [&](const uint32_t* of, int n) {
         __syncthreads();
         if (tid < n) {
-            const uint32_t me = bound_of[tid];
+            const uint32_t me = of[tid];
             int above = 0;
 #pragma unroll 4
             for (int k = 0; k < n; k += 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(bound_of + k);
+                const uint4 x = *reinterpret_cast<const uint4*>(of + k);
                 above += x.x > me, above += x.y > me, above += x.z > me, above += x.w > me;
             }
             if (above == P.num - 1) s_bound = me;
@@ -287,13 +288,22 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
     };
     if (segs >= P.num) {
         if (tid < kSelSegments) bound_of[tid] = record_score(tid, records[tid].m, tid);
-        find_bound(kSelSegments);
+        find_bound(bound_of, kSelSegments);
     }
     if (s_bound <= kMinusInf) {
         if (tid < 4 * kSelSegments) bound_of[tid] = record_score(tid >> 2, records[tid >> 2].quarter[tid & 3], tid);
-        find_bound(4 * kSelSegments);
+        find_bound(bound_of, 4 * kSelSegments);
     }
-    const double bound = s_bound > kMinusInf ? (double)from_ordered32(s_bound & ~kIndexBits) : -CUDART_INF;
+    const bool candidates_here = alive && (done ? seg == 0 : lse[beam] > -CUDART_INF);
+    if (s_bound <= kMinusInf) {
+        // a vocabulary so short, or so few live beams, that less than num quarters hold anything: the maxima of this CTA's lanes bound what
+        // it can contribute (500 tokens of one beam, num 16: without this all of them are candidates: 33 us instead of 18)
+        const double v = candidates_here && m > -CUDART_INF_F && (!done || lane == 0) ? (double)beam_score[beam] + ((double)m - lse[beam]) : -CUDART_INF;
+        const float f = v > -CUDART_INF ? __double2float_rd(v) : -CUDART_INF_F;
+        lane_best[tid] = f > -CUDART_INF_F ? (ordered32(f) & ~(kSelThreads - 1u)) | (uint32_t)tid : (uint32_t)tid;
+        find_bound(lane_best, kSelThreads);
+    }
+    const double bound = s_bound > kMinusInf ? (double)from_ordered32(s_bound & ~(kSelThreads - 1u)) : -CUDART_INF;
 
     // the smallest logit of a beam that can reach the bound, a little lower than it is so that rounding cannot lose one
     auto lowest = [&](int i) -> float {
@@ -315,7 +325,6 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
         cluster_sync_all();
     };
     // pass 2: lanes only note what may reach the bound; the few notes are then weighed side by side, a thread each
-    const bool candidates_here = alive && (done ? seg == 0 : lse[beam] > -CUDART_INF);
     auto note = [&](float x, int t) {
         const unsigned at = atomicAdd(&found_count, 1u);
         if (at < kSelShare) found[at] = make_uint2((unsigned)(beam * vocab + t), __float_as_uint(x));

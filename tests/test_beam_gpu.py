@@ -236,3 +236,20 @@ def test_beam_search_as_it_is_used(dt):
             assert torch.equal(c[:, :, : Lp + t + 1], p)
     assert all(len(set(map(tuple, h))) == N for h in history)   # the beams of a sample are different sequences
     assert (scores[:, :-1] >= scores[:, 1:]).all() and ffa.device_status() == 0
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,beams,V,live", [(1, 1, 500, 1), (3, 1, 2047, 1), (1, 4, 700, 1), (40, 8, 1000, 1), (1, 2, 17, 2), (2, 3, 300, 2), (1, 8, 3001, 2)])
+@pytest.mark.parametrize("num", [1, 9, 16])
+def test_short_vocabularies_and_few_live_beams(dt, B, beams, V, live, num):
+    """Fewer parts that hold anything than candidates to find, with and without ties at the border."""
+    g = torch.Generator().manual_seed(V + num)
+    for ties in (False, True):
+        x = torch.randn(B, beams, V, generator=g)
+        x = ((x * 2).round() if ties else x).to(dt).cuda()
+        scores = -torch.rand(B, beams, generator=g).cuda()
+        scores[:, live:] = float("-inf")
+        finished = torch.zeros(B, beams, dtype=torch.bool, device="cuda")
+        if live > 1:
+            finished[:, 1] = True
+        check(x, scores, num, finished, V - 1)
