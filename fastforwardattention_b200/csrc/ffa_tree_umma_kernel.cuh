@@ -47,6 +47,8 @@ struct UmmaTail {
     uint64_t bars[2 * kUmmaMaxStages + 8];
     uint32_t bad[kTreeMaxRows / 32];   // drafted tokens with an infinity or NaN in V
     uint32_t tmem_base;
+    uint32_t pos[8], neg[8];           // columns with +infinity, -infinity (NaN: both) in a cached V row of this CTA's tiles
+    uint32_t poisoned;                 // groups of 16 columns of O that hold one
     int flags[1];                      // a wait ran out
     int any_bad;
 };
@@ -216,6 +218,31 @@ __device__ __forceinline__ uint32_t nonfinite_mask(uint32_t w)
     return m;
 }
 
+// Notes the columns of those groups of 16 that hold an infinity or NaN in V's cached rows [lo, hi) of the pair: thread `rank` of
+// `threads`.  A product with a weight of 0 (another copy's key, a weight that vanished) has turned such a value into NaN in O.
+template <typename T, int DH>
+__device__ __noinline__ void find_nonfinite(const FfaTreeParams& P, int bh, int lo, int hi, uint32_t groups, uint32_t* pos, uint32_t* neg, int rank, int threads)
+{
+    for (int r = lo + rank; r < hi; r += threads) {
+        const uint4* row = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(P.v_cache) + cache_row_offset(P, bh, r, DH * 2));
+        for (uint32_t g = groups; g != 0; g &= g - 1) {
+            const int first = __ffs(g) - 1;
+            for (int i = 2 * first; i < 2 * first + 2; ++i) {
+                const uint4 x = row[i];
+                if (!(nonfinite_mask<T>(x.x) | nonfinite_mask<T>(x.y) | nonfinite_mask<T>(x.z) | nonfinite_mask<T>(x.w))) continue;
+                float y[8];
+                Elem<T>::unpack(x, y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (isfinite(y[e])) continue;
+                    if (!(y[e] < 0.f)) atomicOr(&pos[i >> 2], 1u << (8 * (i & 3) + e));
+                    if (!(y[e] > 0.f)) atomicOr(&neg[i >> 2], 1u << (8 * (i & 3) + e));
+                }
+            }
+        }
+    }
+}
+
 // the largest of three; NaN if one of them is
 __device__ __forceinline__ float max3_nan(float a, float b, float c)
 {
@@ -266,10 +293,11 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int R = P.groups * P.tokens;
     if (tid == 0) {
-        flags[0] = 0, tail.any_bad = 0;
+        flags[0] = 0, tail.any_bad = 0, tail.poisoned = 0;
         tma_prefetch_map(&U.q), tma_prefetch_map(&U.k_cache), tma_prefetch_map(&U.v_cache), tma_prefetch_map(&U.k_new), tma_prefetch_map(&U.v_new);
     }
     if (tid >= 64 && tid < 64 + kTreeMaxRows / 32) bad[tid - 64] = 0;
+    if (tid >= 96 && tid < 104) tail.pos[tid - 96] = tail.neg[tid - 96] = 0;
     pdl_wait();
     const TreeCut<kUmmaKeys> cut(P);
     const int row0 = cut.rt * P.tile_rows, rows = min(P.tile_rows, R - row0);
@@ -576,20 +604,32 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
             if (ok) {
                 tcgen05_after_sync();
                 float* mine = o_smem + (size_t)(rep * rows + r) * STRIDE;
+                uint32_t poisoned = 0;
 #pragma unroll 1
                 for (int x = 0; x < DH; x += 16) {
                     uint32_t o[16];
                     tmem_ld16<0>(lanes + x, o);
                     tmem_wait_ld(o);
                     if (real) {
+                        float zero = 0.f;   // NaN once one of them is not finite
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) zero = fmaf(0.f, __uint_as_float(o[i]), zero);
+                        if (zero != 0.f) poisoned |= 1u << (x / 16);
 #pragma unroll
                         for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(mine + x + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                     }
                     __syncwarp();
                 }
                 if (real) mine[DH] = m, mine[DH + 1] = l;
+                if (poisoned) atomicOr(&tail.poisoned, poisoned);
             }
             named_bar_sync(1, threads);   // (every warp comes here, also after a wait that ran out)
+            const uint32_t poisoned = tail.poisoned;
+            if (poisoned) {   // (the same for all of them)
+                find_nonfinite<T, DH>(P, cut.bh, max(cut.sr.first, (cut.c0 + cut.u0) * kUmmaKeys),
+                                      min(cut.sr.row, (cut.c0 + min(cut.u1, cut.cache_tiles)) * kUmmaKeys), poisoned, tail.pos, tail.neg, st, threads);
+                named_bar_sync(1, threads);
+            }
             if (ok) {
                 constexpr int OCT = DH / 8;   // eight columns at a time
                 for (int i = st; i < rows * OCT; i += threads) {
@@ -615,7 +655,14 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
                             o[e + 2] = fmaf(w[q], y.z, o[e + 2]), o[e + 3] = fmaf(w[q], y.w, o[e + 3]);
                         }
                     }
-                    if (tail.any_bad) {   // a visible infinity or NaN decides its column
+                    if (poisoned) {   // an infinity or NaN in a cached row decides its column, whatever its weight
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const bool up = (tail.pos[x >> 5] >> ((x & 31) + e)) & 1, down = (tail.neg[x >> 5] >> ((x & 31) + e)) & 1;
+                            if (up || down) o[e] = up && down ? CUDART_NAN_F : up ? CUDART_INF_F : -CUDART_INF_F;
+                        }
+                    }
+                    if (tail.any_bad) {   // and so does one in a drafted token that the row sees
                         const T* v = static_cast<const T*>(P.v) + (size_t)cut.bh * P.tokens * DH + x;
                         const unsigned char* sees = tree + (size_t)((row0 + row) % P.tokens) * P.tokens;
                         for (int k = 0; k < P.tokens; ++k) {

@@ -183,6 +183,8 @@ int ffa_attention_paged(ffa_plan_t* plan, const void* q, const void* k, const vo
  * t, seq_lengths and right_or_no_padding mean what they mean in ffa_attention (with per-sample lengths a sample that lies above
  * the bound t or has no room for its tokens is refused: FFA_STATUS_BAD_LENGTH, output zero, nothing appended).
  * A query row that sees nothing is 0.  A token that a row does not see has no influence on it, whatever its values.
+ * An infinity in a visible row of V, cached or drafted, is one in the result (fp32: as long as the row's weight is a number of fp32 above
+ * 0), infinities of both signs or NaN are NaN.
  * Statistics and sums are fp32; fp16 and bf16 weights are rounded to the tensors' type before they meet V, and the result once.
  * groups * tokens <= 1024.  page_table: NULL, or the paged caches of ffa_attention_paged with pools of pool_pages pages; every page
  * that holds rows 0..row+tokens-1 of a sequence has to be in its table (a sequence with an entry outside [0, pool_pages) there is

@@ -1,5 +1,5 @@
 """Attention of a tree of drafted tokens over a cache, and the acceptance of a path, against their 64-bit definitions."""
-import pytest
+import math
 import torch
 
 from oracle import decoding_oracle as D64
@@ -447,3 +447,21 @@ def test_pages_that_are_missing_or_outside_the_pool_are_refused(dt):
     # rows 133, 134 -> 130, 131 lie in the second one (page 5, rows 5, 6 -> 2, 3)
     kb[5, :, 2:4] = kb[5, :, 5:7].clone()
     assert torch.equal(pool.k[0, :, 121], kb[1, :, 11]) and torch.equal(pool.k[2:], kb[2:])
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("D", [64, 80, 256])
+@pytest.mark.parametrize("T", [1, 8, 40, 100])
+@pytest.mark.parametrize("n", [130, 5000])
+def test_an_infinity_in_a_cached_row_is_one_in_the_result(dt, D, T, n):
+    """Every row sees it with a weight above 0, however many rows share the key tiles and however many CTAs the pair."""
+    ffa, kc, vc, q, k, v, tree = setup(dt, 2, 2, 1, D, n, T, seed=D + T + n)
+    q *= 0.5   # (fp32 weights do not vanish: scores stay within a few dozen)
+    vc[0, 0, 3, 5], vc[0, 0, n - 1, D - 1] = float("inf"), -float("inf")
+    vc[0, 1, 64, 17], vc[0, 1, 100, 17] = float("inf"), -float("inf")   # of both signs: NaN
+    vc[1, 0, 65, 30], vc[1, 0, 2, 31] = float("nan"), float("inf")
+    v[0, 0, 0, 6] = -float("inf")                                        # and one in a drafted token, next to a cached one's column
+    want, bound = D64.tree_attention(q, k, v, kc, vc, tree, D ** -0.5, [n, n])
+    assert torch.isinf(want[0, 0, :, 5]).all() and torch.isnan(want[0, 1, :, 17]).all() and torch.isfinite(want[1, 1]).all()
+    out = ffa.tree_attention(q, k, v, tree, D ** -0.5, n)
+    D64.assert_within(out, want, bound)
