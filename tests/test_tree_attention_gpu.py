@@ -1,5 +1,5 @@
 """Attention of a tree of drafted tokens over a cache, and the acceptance of a path, against their 64-bit definitions."""
-import math
+import pytest
 import torch
 
 from oracle import decoding_oracle as D64
