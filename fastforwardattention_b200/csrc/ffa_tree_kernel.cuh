@@ -608,12 +608,12 @@ __global__ void __launch_bounds__(256) ffa_tree_accept_kernel(const FfaAcceptPar
     for (; count < P.path_len; ++count) {
         const int j = path[count];
         if (j < 0) break;
-        bool missing = false;
-        if (P.page_table != nullptr && j >= 0 && j < P.Lmax - n) {   // the row itself and the one it moves to
+        bool refused = j <= prev || j >= P.Lmax - n;
+        if (!refused && P.page_table != nullptr) {   // the row itself and the one it moves to: an increasing path has count <= j, so both lie in the table
             const int from = P.page_table[(size_t)b * P.max_pages + (n + j) / P.page_rows], to = P.page_table[(size_t)b * P.max_pages + (n + count) / P.page_rows];
-            missing = from < 0 || from >= P.pool_pages || to < 0 || to >= P.pool_pages;
+            refused = from < 0 || from >= P.pool_pages || to < 0 || to >= P.pool_pages;
         }
-        if (j <= prev || j >= P.Lmax - n || missing) {
+        if (refused) {
             if (threadIdx.x == 0) atomicOr(P.status, kStatusBadIndex);
             return;
         }

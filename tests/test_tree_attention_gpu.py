@@ -512,3 +512,21 @@ def test_many_light_keys_beside_a_heavy_one(dt, T, units):
     want, bound = close_bound(*map(last, (q, k, v, kc, vc)), tree, scale, [n])
     out = ffa.tree_attention(q, k, v, tree, scale, n)
     D64.assert_within(last(out), want, bound)
+
+
+def test_paths_that_repeat_an_index_at_the_end_of_a_paged_sequence():
+    """The last row of the last sequence has no table entry behind it: such a path is refused before its pages are looked up."""
+    from fastforwardattention_b200 import PagePool, _extension
+
+    B, H, D, pr = 2, 2, 64, 128
+    pool = PagePool(4, H, D, torch.float16, "cuda", page_rows=pr)
+    pool.k.normal_(), pool.v.normal_()
+    kb, vb = pool.k.clone(), pool.v.clone()
+    engine = _extension().PagedEngine(pool.k, pool.v, B, 2)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    last = torch.tensor([2 * pr - 1] * B, dtype=torch.int32, device="cuda")
+    for path in ([[0, 0], [0, 0]], [[0, 0, 0, 0]] * 2, [[0, 1], [0, 1]]):
+        engine.tree_accept_per_sample(torch.tensor(path, dtype=torch.int32, device="cuda"), table, last)
+        assert engine.device_status() == 4 and torch.equal(pool.k, kb) and torch.equal(pool.v, vb)
+    engine.tree_accept_per_sample(torch.tensor([[0, -1], [0, -1]], dtype=torch.int32, device="cuda"), table, last)
+    assert engine.device_status() == 0 and torch.equal(pool.k, kb)
