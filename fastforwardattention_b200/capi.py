@@ -14,7 +14,7 @@ F32, F16, BF16 = 0, 1, 2
 MODE_EXACT, MODE_ROUND_LIKE_TORCH = 0, 1
 
 SYMBOLS = ["ffa_cache_bytes", "ffa_cache_init", "ffa_plan_create", "ffa_plan_destroy", "ffa_plan_get_launch",
-           "ffa_plan_set_launch", "ffa_plan_set_mode", "ffa_workspace_bytes", "ffa_workspace_bind", "ffa_attention",
+           "ffa_plan_set_launch", "ffa_plan_set_mode", "ffa_workspace_bytes", "ffa_workspace_bind", "ffa_workspace_score_bytes", "ffa_workspace_bind_scores", "ffa_attention",
            "ffa_device_status", "ffa_launch_count", "ffa_last_error", "ffa_attention_static_scratch", "ffa_static_scratch_status", "ffa_static_scratch_selftest_wait_timeout", "ffa_selftest_wait_timeout", "ffa_plan_set_prune_path", "ffa_plan_create_offline",
            "ffa_plan_get_prune_launch", "ffa_plan_get_prune_path", "ffa_cache_copy", "ffa_attention_paged", "ffa_peer_gather_bytes",
            "ffa_peer_mem_alloc", "ffa_peer_mem_open", "ffa_peer_mem_close", "ffa_peer_mem_free", "ffa_peer_gather_attach",
@@ -61,6 +61,9 @@ def lib() -> C.CDLL:
         L.ffa_workspace_bytes.argtypes = [vp, i]
         L.ffa_workspace_bytes.restype = sz
         L.ffa_workspace_bind.argtypes = [vp, vp, sz, vp]
+        L.ffa_workspace_score_bytes.argtypes = [vp]
+        L.ffa_workspace_score_bytes.restype = sz
+        L.ffa_workspace_bind_scores.argtypes = [vp, vp, sz]
         L.ffa_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, f, i, vp, i, f, vp, vp]
         L.ffa_attention_paged.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, i, vp, f, i, vp, i, f, vp, vp]
         L.ffa_device_status.argtypes = [vp, vp, C.POINTER(i)]

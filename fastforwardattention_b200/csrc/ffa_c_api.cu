@@ -563,6 +563,22 @@ int ffa_workspace_bind(ffa_plan_t* plan, void* workspace, size_t bytes, void* st
     return FFA_OK;
 }
 
+size_t ffa_workspace_score_bytes(const ffa_plan_t* plan)
+{
+    return plan == nullptr ? 0 : carve(plan, true).total - carve(plan, false).total;
+}
+
+int ffa_workspace_bind_scores(ffa_plan_t* plan, void* scores, size_t bytes)
+{
+    if (plan == nullptr || scores == nullptr) return fail(FFA_ERR_ARG, "null pointer");
+    if (plan->ws == nullptr) return fail(FFA_ERR_WORKSPACE, "no workspace bound (ffa_workspace_bind)");
+    if ((reinterpret_cast<uintptr_t>(scores) & 255u) != 0) return fail(FFA_ERR_ARG, "the scores must be 256-byte aligned");
+    const size_t need = ffa_workspace_score_bytes(plan);
+    if (bytes < need) return fail(FFA_ERR_WORKSPACE, "scores of %zu bytes, need at least %zu", bytes, need);
+    plan->scores = static_cast<float*>(scores);   // written before they are read, by every step that uses them
+    return FFA_OK;
+}
+
 namespace {
 
 // a half of a rank's staging buffer for the output gather: [B][world][H * Dh] elements

@@ -121,6 +121,29 @@ void run_accept(const TreeTarget& T, const torch::Tensor& path_, int64_t t, cons
           "tree accept");
 }
 
+// An engine's device memory beside its caches.  The score scratch (4 bytes a cache row) comes when a step first asks for it and lies beside the
+// workspace, which is never replaced: graphs recorded before hold its counters, and its status word collects their bits.
+struct Workspace {
+    torch::Tensor base, scores;
+    void bind(ffa_plan_t* plan, c10::Device device)
+    {
+        const size_t n = ffa_workspace_bytes(plan, 0);
+        base = torch::empty({(int64_t)n}, torch::TensorOptions().dtype(torch::kUInt8).device(device)), scores = torch::Tensor();
+        check(ffa_workspace_bind(plan, base.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()), "workspace");
+    }
+    void bind_scores(ffa_plan_t* plan, c10::Device device, const char* who)
+    {
+        if (scores.defined()) return;
+        cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+        cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing);
+        TORCH_CHECK(capturing == cudaStreamCaptureStatusNone, who,
+                    ": make the first pruned or accumulating step outside of a graph capture: it allocates the score scratch, which is not one graph's");
+        const size_t n = ffa_workspace_score_bytes(plan);
+        scores = torch::empty({(int64_t)n}, torch::TensorOptions().dtype(torch::kUInt8).device(device));
+        check(ffa_workspace_bind_scores(plan, scores.data_ptr(), n), "score scratch");
+    }
+};
+
 struct FastForwardAttn {
     FastForwardAttn(torch::Tensor K, torch::Tensor V, int64_t max_timesteps, bool use_default_kernel_launch)
     {
@@ -145,7 +168,7 @@ struct FastForwardAttn {
         check(ffa_cache_init(dtype, (int)B, (int)H, (int)Lp, (int)Lmax, (int)Dh, K.data_ptr(), V.data_ptr(), k_cache.data_ptr(),
                              v_cache.data_ptr(), stream.stream()),
               "cache init");
-        bind_workspace(false);
+        ws.bind(plan, device);
         // one-time: the caches and the cleared workspace are complete before the constructor
         // returns, so the first step may run on any stream
         stream.synchronize();
@@ -167,7 +190,7 @@ struct FastForwardAttn {
         use_default = use_default_kernel_launch;
         check(ffa_plan_create(dtype, (int)B, (int)H, (int)Dh, (int)Lmax, use_default, device.index(), &plan), "plan");
         k_cache = kc, v_cache = vc;
-        bind_workspace(false);
+        ws.bind(plan, device);
         at::cuda::getCurrentCUDAStream().synchronize();
     }
 
@@ -197,11 +220,16 @@ struct FastForwardAttn {
             check(ffa_peer_gather_attach(np, peer_world, peer_rank, bufs.data(), peer_bytes), "peer gather");
         }
         stream.synchronize();   // the old slabs may be freed once the copy is done
+        int before = 0;         // and so may the old workspace with its status word
+        ffa_device_status(plan, stream.stream(), &before);
+        status_before |= before;
         ffa_plan_destroy(plan);
         plan = np, k_cache = nk, v_cache = nv, Lmax = new_max_len;
         kept_mask = torch::Tensor();   // one bit per row of the old length; re-created on the next recorded call
         push_tensor = torch::Tensor();
-        bind_workspace(has_scores);
+        const bool with_scores = ws.scores.defined();
+        ws.bind(plan, device);
+        if (with_scores) ws.bind_scores(plan, device, "FastForwardAttn");
         stream.synchronize();
     }
     int64_t max_len() const { return Lmax; }
@@ -213,14 +241,6 @@ struct FastForwardAttn {
     }
     FastForwardAttn(const FastForwardAttn&) = delete;
     FastForwardAttn& operator=(const FastForwardAttn&) = delete;
-
-    void bind_workspace(bool with_scores)
-    {
-        const size_t n = ffa_workspace_bytes(plan, with_scores);
-        workspace = torch::empty({(int64_t)n}, torch::TensorOptions().dtype(torch::kUInt8).device(device));
-        check(ffa_workspace_bind(plan, workspace.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()), "workspace");
-        has_scores = with_scores;
-    }
 
     // memory the engine's kernels can address: its own device, or pinned (page-locked) host memory
     bool reachable(const torch::Tensor& x) const { return (x.is_cuda() && x.device() == device) || (x.is_cpu() && x.is_pinned()); }
@@ -277,7 +297,7 @@ struct FastForwardAttn {
         // large pruned steps go through an fp32 score scratch (4 bytes per cache row, under 1 % of the caches): bound
         // the first time a pruned step is asked for.  (Torch-rounding steps keep their scores in shared memory; the
         // retry below binds the scratch for the rare shape that does not fit there.)
-        if (p > 0.0 && !has_scores) bind_workspace(true);
+        if (p > 0.0) ws.bind_scores(plan, device, "FastForwardAttn");
         auto call = [&]() {
             return ffa_attention(plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(),
                                  (float)softmax_scale, (int)t, seq_lengths ? sl.data_ptr<int>() : nullptr, right_or_no_padding,
@@ -296,9 +316,9 @@ struct FastForwardAttn {
             }
         }
         int rc = call();
-        if (rc == FFA_ERR_WORKSPACE && !has_scores) {
-            // a shape the fused pruning kernel cannot hold: grow the workspace by the score scratch, once
-            bind_workspace(true);
+        if (rc == FFA_ERR_WORKSPACE && !ws.scores.defined()) {
+            // a shape the fused pruning kernel cannot hold: add the score scratch, once
+            ws.bind_scores(plan, device, "FastForwardAttn");
             rc = call();
         }
         if (pushed) ffa_peer_push_target(plan, nullptr);
@@ -411,14 +431,7 @@ struct FastForwardAttn {
         torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({B, H, Dh}, k_cache.options());
         TORCH_CHECK(out.is_cuda() && out.device() == device && dtype_code(out) == dtype && out.is_contiguous() && out.numel() == n,
                     "FastForwardAttn: out must be a contiguous tensor of batch*heads*head_dim elements on the engine's device");
-        if (!has_scores) {   // once, as for pruned steps
-            cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-            cudaStreamIsCapturing(at::cuda::getCurrentCUDAStream().stream(), &capturing);
-            TORCH_CHECK(capturing == cudaStreamCaptureStatusNone,
-                        "FastForwardAttn: make the first accumulating step outside of a graph capture: it binds the score scratch");
-            retired.push_back(workspace);   // graphs recorded before go on using it
-            bind_workspace(true);
-        }
+        ws.bind_scores(plan, device, "FastForwardAttn");   // once, as for pruned steps
         check(ffa_attention_accumulate(plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(),
                                        (float)softmax_scale, (int)(max_row < 0 ? Lmax - 1 : max_row), rows.data_ptr<int>(),
                                        weights.data_ptr<float>(), positions.data_ptr<int>(), seen.data_ptr<int>(),
@@ -506,6 +519,7 @@ struct FastForwardAttn {
         int s = 0;
         const int rc = ffa_device_status(plan, at::cuda::getCurrentCUDAStream().stream(), &s);
         TORCH_CHECK(rc == FFA_OK || rc == FFA_ERR_DEVICE, "FastForwardAttn: status: ", ffa_last_error());
+        s |= status_before, status_before = 0;
         return s;
     }
 
@@ -591,12 +605,13 @@ struct FastForwardAttn {
     }
 
     ffa_plan_t* plan = nullptr;
-    torch::Tensor k_cache, v_cache, workspace, kept_mask, push_tensor;
-    std::vector<torch::Tensor> retired;   // workspaces that recorded graphs may hold
+    torch::Tensor k_cache, v_cache, kept_mask, push_tensor;
+    Workspace ws;
+    int status_before = 0;   // bits of the status word that grow() replaced
     c10::Device device{c10::kCUDA, 0};
     int64_t B = 0, H = 0, Dh = 0, Lmax = 0;
     int dtype = 0, mode = FFA_MODE_EXACT, prune_path = 0;
-    bool has_scores = false, want_mask = false, use_default = false, cluster_merge = true, launch_forced = false;
+    bool want_mask = false, use_default = false, cluster_merge = true, launch_forced = false;
     ffa_launch_t forced_launch{};
     void* peer_own = nullptr;
     std::vector<void*> peer_ptrs;
@@ -625,17 +640,10 @@ struct PagedEngine {
         c10::cuda::CUDAGuard guard(device);
         check(ffa_plan_create(dtype, (int)B, (int)H, (int)Dh, (int)(max_pages * page_rows), use_default_kernel_launch, device.index(), &plan),
               "plan");
-        bind_workspace(false);
+        ws.bind(plan, device);
         at::cuda::getCurrentCUDAStream().synchronize();
     }
     ~PagedEngine() { ffa_plan_destroy(plan); }
-    void bind_workspace(bool with_scores)
-    {
-        const size_t n = ffa_workspace_bytes(plan, with_scores);
-        workspace = torch::empty({(int64_t)n}, torch::TensorOptions().dtype(torch::kUInt8).device(device));
-        check(ffa_workspace_bind(plan, workspace.data_ptr(), n, at::cuda::getCurrentCUDAStream().stream()), "workspace");
-        has_scores = with_scores;
-    }
     PagedEngine(const PagedEngine&) = delete;
     PagedEngine& operator=(const PagedEngine&) = delete;
 
@@ -670,7 +678,7 @@ struct PagedEngine {
                 kept_mask = torch::zeros({B, H, (max_pages * page_rows + 31) / 32}, torch::TensorOptions().dtype(torch::kInt).device(device));
             mask_ptr = reinterpret_cast<uint32_t*>(kept_mask.data_ptr());
         }
-        if (p > 0.0 && !has_scores) bind_workspace(true);   // torch-rounding steps keep their scores in shared memory
+        if (p > 0.0) ws.bind_scores(plan, device, "PagedEngine");   // torch-rounding steps keep their scores in shared memory
         auto call = [&]() {
             return ffa_attention_paged(plan, q.data_ptr(), k.data_ptr(), v.data_ptr(), kp.data_ptr(), vp.data_ptr(),
                                        table.data_ptr<int>(), (int)max_pages, (int)page_rows, out.data_ptr(), (float)softmax_scale,
@@ -678,9 +686,9 @@ struct PagedEngine {
                                        at::cuda::getCurrentCUDAStream().stream());
         };
         int rc = call();
-        if (rc == FFA_ERR_WORKSPACE && !has_scores) {
-            // a shape the fused pruning kernel cannot hold: grow the workspace by the score scratch, once
-            bind_workspace(true);
+        if (rc == FFA_ERR_WORKSPACE && !ws.scores.defined()) {
+            // a shape the fused pruning kernel cannot hold: add the score scratch, once
+            ws.bind_scores(plan, device, "PagedEngine");
             rc = call();
         }
         check(rc, "paged attention");
@@ -734,11 +742,12 @@ struct PagedEngine {
     }
 
     ffa_plan_t* plan = nullptr;
-    torch::Tensor kp, vp, workspace, kept_mask;
+    torch::Tensor kp, vp, kept_mask;
+    Workspace ws;
     c10::Device device{c10::kCUDA, 0};
     int64_t B = 0, H = 0, Dh = 0, page_rows = 0, max_pages = 0;
     int dtype = 0, mode = FFA_MODE_EXACT;
-    bool has_scores = false, want_mask = false;
+    bool want_mask = false;
 };
 
 // Selection over beams and vocabulary (ffa_beam_select): (scores fp32, parents int32, tokens int32), each [batch, num].

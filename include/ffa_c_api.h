@@ -135,9 +135,13 @@ int ffa_plan_get_prune_path(const ffa_plan_t* plan, int t, float p, int with_sco
  * word and, when with_scores != 0 (needed for p > 0 and FFA_MODE_ROUND_LIKE_TORCH), one fp32
  * score per cache row (the streaming pruning kernel's scratch; ffa_attention returns
  * FFA_ERR_WORKSPACE if a call needs it and it is missing).  The caller allocates it (256-byte aligned) and binds it once;
- * binding clears the counters on the stream.  One workspace serves one stream at a time. */
+ * binding clears the counters on the stream.  One workspace serves one stream at a time.
+ * A plan whose workspace came without the scores gets them later from ffa_workspace_bind_scores: ffa_workspace_score_bytes of device memory,
+ * 256-byte aligned, beside the workspace, which stays as it is -- counters, status word and the graphs that were recorded with it. */
 size_t ffa_workspace_bytes(const ffa_plan_t* plan, int with_scores);
 int ffa_workspace_bind(ffa_plan_t* plan, void* workspace, size_t bytes, void* stream);
+size_t ffa_workspace_score_bytes(const ffa_plan_t* plan);
+int ffa_workspace_bind_scores(ffa_plan_t* plan, void* scores, size_t bytes);
 
 /* One decode step.  q, k, v: batch*heads*head_dim contiguous elements in (batch, head, dim)
  * order.  Writes k and v into row `row` of the caches and out[batch, heads, head_dim], where

@@ -113,3 +113,16 @@ def test_peer_gather_arguments_without_gpu():
     assert L.ffa_peer_mem_open(None, C.byref(g)) == -4
     assert L.ffa_peer_mem_close(None) == 0 and L.ffa_peer_mem_free(None) == 0
     L.ffa_plan_destroy(p)
+
+
+def test_score_scratch_sizes_and_refusals():
+    L = capi.lib()
+    p = C.c_void_p()
+    capi.check(L.ffa_plan_create_offline(capi.F16, 2, 4, 64, 1000, 0, 148, 232448, 233472, C.byref(p)))
+    n = L.ffa_workspace_score_bytes(p)
+    assert n == L.ffa_workspace_bytes(p, 1) - L.ffa_workspace_bytes(p, 0) and n >= 2 * 4 * 1000 * 4
+    assert L.ffa_workspace_score_bytes(None) == 0
+    assert L.ffa_workspace_bind_scores(None, C.c_void_p(4096), n) == -4
+    assert L.ffa_workspace_bind_scores(p, None, n) == -4
+    assert L.ffa_workspace_bind_scores(p, C.c_void_p(4096), n) == -6   # the workspace comes first
+    L.ffa_plan_destroy(p)
