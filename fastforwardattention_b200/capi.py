@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libffa_b200
 F32, F16, BF16 = 0, 1, 2
 MODE_EXACT, MODE_ROUND_LIKE_TORCH = 0, 1
 
-SYMBOLS = ["ffa_cache_bytes", "ffa_cache_init", "ffa_plan_create", "ffa_plan_destroy", "ffa_plan_get_launch",
+SYMBOLS = ["ffa_cache_bytes", "ffa_cache_init", "ffa_plan_create", "ffa_plan_destroy", "ffa_plan_get_launch", "ffa_plan_get_accumulate_launch",
            "ffa_plan_set_launch", "ffa_plan_set_mode", "ffa_workspace_bytes", "ffa_workspace_bind", "ffa_workspace_score_bytes", "ffa_workspace_bind_scores", "ffa_attention",
            "ffa_device_status", "ffa_launch_count", "ffa_last_error", "ffa_attention_static_scratch", "ffa_static_scratch_status", "ffa_static_scratch_selftest_wait_timeout", "ffa_selftest_wait_timeout", "ffa_plan_set_prune_path", "ffa_plan_create_offline",
            "ffa_plan_get_prune_launch", "ffa_plan_get_prune_path", "ffa_cache_copy", "ffa_attention_paged", "ffa_peer_gather_bytes",
@@ -54,6 +54,7 @@ def lib() -> C.CDLL:
         L.ffa_plan_destroy.argtypes = [vp]
         L.ffa_plan_destroy.restype = None
         L.ffa_plan_get_launch.argtypes = [vp, i, C.POINTER(Launch)]
+        L.ffa_plan_get_accumulate_launch.argtypes = [vp, i, C.POINTER(Launch)]
         L.ffa_plan_set_launch.argtypes = [vp, C.POINTER(Launch)]
         L.ffa_plan_set_mode.argtypes = [vp, i]
         L.ffa_plan_set_prune_path.argtypes = [vp, i]

@@ -126,11 +126,14 @@ Shape measured_shape(const ffa_plan* p, int row_bytes, long long rows_total, int
     if (tensors == 1) return s;   // the refinements below were measured on the exact kernel (K and V tiles)
     const double bytes = (double)rows_total * row_bytes * tensors;
     const long long BH = (long long)p->B * p->H;
-    if (p->accumulating && bytes >= 500e6) {
-        // accumulating steps pause at the end of every pair to add its weights: twice the warps do that in half the time, and a third
-        // stage keeps HBM busier meanwhile (bf16 x 128, 1024 pairs x 2047 rows: 184.5 -> 171.7 us; 256 pairs x 4000: 90.9 -> 87.7;
-        // 1024 pairs x 500, 262 MB: 50.9 against 53.7)
-        s.warps = 8, s.stages = 3;
+    if (p->accumulating && bytes >= 500e6 && p->Dh != 80) {
+        // accumulating steps pause at the end of every pair to add its weights: a third stage keeps HBM busier meanwhile, and twice the warps do it
+        // in half the time where a tile has rows for all their lane groups (1024-byte rows: 16 rows for 4 warps, 8 for 8).  Four warps and two stages /
+        // four and three / eight and three, 1024 pairs and 128 pairs of 1.2 GB: fp16 x 64 221 / 214 / 206 and 218 / 209 / 207 us, fp16 x 128
+        // 216 / 205 / 199 and 213 / 203 / 197, fp16 x 256 218 / 209 / 195 and 213 / 203 / 193, fp32 x 128 199 / 195 / 188 and 203 / 192 / 191, fp32 x 256
+        // 211 / 200 / 219 and 202 / 191 / 215; at 0.52 GB the same order.  (bf16 x 128, 1024 pairs x 500, 262 MB: eight and three lose, 53.7
+        // against 50.9.)  Head_dim 80 keeps four warps and two stages (228 / 228 / 508 and 208 / 209 / 514 us): see stream_ctas_by_registers.
+        s.warps = row_bytes > 512 ? 4 : 8, s.stages = 3;
         return s;
     }
     if (bytes < 48e6) {
@@ -156,6 +159,11 @@ Shape measured_shape(const ffa_plan* p, int row_bytes, long long rows_total, int
     return s;
 }
 
+// Resident CTAs of the exact and the accumulating kernel per SM that its registers leave room for.  Only head_dim 80 is short of them: 168 a
+// thread (five vectors of a row in flight) are two CTAs of five warps or one of nine; a grid of more runs in waves (accumulating steps, fp16 x 80,
+// 1024 pairs x 1586 rows with nine warps: 288 us, with five 122; exact steps of 600 pairs x 100 rows at four CTAs to an SM: 32.2 us, at two 19.7).
+int stream_ctas_by_registers(const ffa_plan* p, int warps) { return p->Dh == 80 ? 65536 / (168 * 32 * (warps + 1)) : kMaxCtasPerSm; }
+
 int fit_launch(const ffa_plan* p, int cap_rows, int tensors, ffa_launch_t* out, bool pow2_tiles = false, int max_parts = 0)
 {
     const int rowb = p->Dh * elem_size(p->dtype);
@@ -172,8 +180,10 @@ int fit_launch(const ffa_plan* p, int cap_rows, int tensors, ffa_launch_t* out, 
     if (s.warps > 8) s.warps = 8;   // the kernels are compiled for at most 1 + 8 warps
     if (tensors == 1 && p->Dh == 80 && s.warps > 4) s.warps = 4;   // streaming pruning kernel, five vectors per lane: register budget
     if (tensors == 1 && s.cps > 2) s.cps = 2;   // its 13 warps of 72 registers leave room for two CTAs per SM
+    const bool cps_forced = p->forced && p->force.ctas_per_sm > 0;
+    const int most_cps = tensors == 2 && !cps_forced ? stream_ctas_by_registers(p, s.warps) : kMaxCtasPerSm;
+    if (s.cps > most_cps) s.cps = most_cps;
     if (s.cps < 1) s.cps = 1;
-    if (s.cps > kMaxCtasPerSm) s.cps = kMaxCtasPerSm;
     if (s.stages < 2) s.stages = 2;
     if (s.stages > 16) s.stages = 16;
     if (s.tile_rows < 8) s.tile_rows = 8;
@@ -240,7 +250,7 @@ int fit_launch(const ffa_plan* p, int cap_rows, int tensors, ffa_launch_t* out, 
         } else {
             const int need = (int)((BH + p->sms - 1) / p->sms);
             const int smem = out->smem_bytes;
-            if (need <= 4 && (long long)need * (smem + kSmemReservePerCta) <= p->smem_per_sm && !(p->forced && p->force.ctas_per_sm > 0)) {
+            if (need <= 4 && need <= most_cps && (long long)need * (smem + kSmemReservePerCta) <= p->smem_per_sm && !cps_forced) {
                 s.cps = need, parts = 1, grid = BH;
             } else {
                 // more pairs than slots: k whole pairs per persistent CTA, nothing straddles; its copy warp streams across
@@ -506,6 +516,15 @@ int ffa_plan_get_launch(const ffa_plan_t* plan, int t, ffa_launch_t* launch)
     if (r != FFA_OK) return r;
     int cluster = 0;
     return fit_clusters(const_cast<ffa_plan_t*>(plan), t, false, launch, &cluster);   // fills the plan's occupancy cache
+}
+
+int ffa_plan_get_accumulate_launch(ffa_plan_t* plan, int t, ffa_launch_t* launch)
+{
+    if (plan == nullptr) return fail(FFA_ERR_ARG, "null pointer");
+    plan->accumulating = true;
+    const int r = ffa_plan_get_launch(plan, t, launch);
+    plan->accumulating = false;
+    return r;
 }
 
 int ffa_plan_set_launch(ffa_plan_t* plan, const ffa_launch_t* launch)

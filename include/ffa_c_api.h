@@ -99,8 +99,9 @@ int ffa_plan_create_offline(int dtype, int batch, int heads, int head_dim, int m
                             int smem_per_cta, int smem_per_sm, ffa_plan_t** plan);
 void ffa_plan_destroy(ffa_plan_t* plan);
 
-/* The launch shape the planner picks for step t (after any override). */
+/* The launch shape the planner picks for step t (after any override), and for an accumulating step (ffa_attention_accumulate). */
 int ffa_plan_get_launch(const ffa_plan_t* plan, int t, ffa_launch_t* launch);
+int ffa_plan_get_accumulate_launch(ffa_plan_t* plan, int t, ffa_launch_t* launch);
 /* Forces a launch shape (fields <= 0 keep the planner's choice); NULL removes the override.
  * Used by the tuning sweep; the reference exposes tpb/tpv/tpk the same way
  * (c_ffa_api.h:17-20). */

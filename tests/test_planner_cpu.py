@@ -163,3 +163,45 @@ def test_which_pruning_kernel_a_step_takes():
     L, p = offline(capi.F32, 1, 1, 64, 2000000)
     assert prune_path(L, p, 1999999, 1e-3) == 2
     assert prune_path(L, p, 1999999, 1e-3, with_scores=0) == 0
+
+
+REGISTERS = {80: 168}   # a thread of the exact and accumulating kernels (ptxas); the other head sizes are compiled for at most 96
+
+
+def accumulate_launch(L, p, t):
+    l = capi.Launch()
+    capi.check(L.ffa_plan_get_accumulate_launch(p, t, C.byref(l)))
+    return l
+
+
+@pytest.mark.parametrize("dtype,Dh", list(itertools.product([capi.F32, capi.F16, capi.BF16], [64, 80, 128, 256])))
+def test_accumulating_steps_leave_registers_for_every_resident_cta(dtype, Dh):
+    """A grid of one CTA per slot has to be resident at once: more CTAs to an SM than its 65536 registers hold run in waves."""
+    for pairs, rows in [(1024, 300), (1024, 1600), (1024, 4000), (128, 12000), (256, 9000)]:
+        L, p = offline(dtype, pairs // 32, 32, Dh, rows + 1)
+        l = accumulate_launch(L, p, rows)
+        assert l.ctas_per_sm * 32 * (l.consumer_warps + 1) * REGISTERS.get(Dh, 96) <= 65536, (pairs, rows)
+        assert l.smem_bytes <= SMEM_CTA and l.ctas_per_sm * (l.smem_bytes + 1024) <= SMEM_SM
+        L.ffa_plan_destroy(p)
+
+
+@pytest.mark.parametrize("dtype", [capi.F32, capi.F16, capi.BF16])
+@pytest.mark.parametrize("get", [launch, accumulate_launch])
+def test_head_dim_80_takes_at_most_two_ctas_to_an_sm(dtype, get):
+    for pairs in (1, 40, 160, 320, 450, 600, 1024, 2016):
+        for rows in (1, 30, 100, 300, 1200, 4000):
+            L, p = offline(dtype, 1, pairs, 80, rows + 1)
+            l = get(L, p, rows)
+            assert l.ctas_per_sm * 32 * (l.consumer_warps + 1) * 168 <= 65536 and l.grid <= 2 * SMS, (pairs, rows)
+            L.ffa_plan_destroy(p)
+
+
+def test_accumulating_shapes_by_size():
+    """Eight warps and three stages from 500 MB, four and three for 1024-byte rows, the plain step's shape otherwise and for head_dim 80."""
+    for dtype, Dh, rows, want in [(capi.BF16, 128, 2047, (8, 3)), (capi.F16, 64, 4000, (8, 3)), (capi.F16, 256, 1100, (8, 3)), (capi.F32, 256, 570, (4, 3)),
+                                  (capi.F16, 80, 3600, (4, 2)), (capi.F32, 80, 1800, (4, 2)), (capi.BF16, 128, 600, (4, 2))]:
+        L, p = offline(dtype, 32, 32, Dh, rows + 1)
+        l = accumulate_launch(L, p, rows)
+        assert (l.consumer_warps, l.stages) == want, (dtype, Dh)
+        L.ffa_plan_destroy(p)
+    assert L.ffa_plan_get_accumulate_launch(None, 0, C.byref(l)) == -4
