@@ -72,6 +72,7 @@ class PagedFastForwardAttn:
         self.table = self.table_host.to(dev)
         self.rows = torch.tensor(self.lengths, dtype=torch.int32, device=dev)
         self.engine = _extension().PagedEngine(pool.k, pool.v, B, self.max_pages, use_default_kernel_launch)
+        self.drafted = 0   # tokens of the last tree, behind every sequence's rows until they are accepted or overwritten
 
     def _ensure_page(self, b: int, row: int) -> None:
         i = row // self.pool.page_rows
@@ -91,6 +92,7 @@ class PagedFastForwardAttn:
                 self._ensure_page(b, n)
         res = self.engine.attention_per_sample(q, k, v, self.table, softmax_scale, self.rows, prob_thresh, out=out,
                                                max_row=max(self.lengths))
+        self.drafted = 0
         self.rows += 1
         self.lengths = [n + 1 for n in self.lengths]
         return res
@@ -106,19 +108,21 @@ class PagedFastForwardAttn:
         for b, n in enumerate(self.lengths):
             for row in range(n // self.pool.page_rows * self.pool.page_rows, n + T, self.pool.page_rows):
                 self._ensure_page(b, row)
-        return self.engine.tree_attention_per_sample(q, k, v, tree, self.table, softmax_scale, self.rows, out=out,
-                                                     max_row=max(self.lengths))
+        res = self.engine.tree_attention_per_sample(q, k, v, tree, self.table, softmax_scale, self.rows, out=out,
+                                                    max_row=max(self.lengths))
+        self.drafted = T
+        return res
 
     def tree_accept(self, path: Sequence[Sequence[int]]) -> None:
-        """Keeps path[b] (increasing indices into the tree of the last tree_attention) of every sequence: its rows move to the
-        end of the sequence, which grows by len(path[b]).  Pages taken for the rest of the tree stay with the sequence."""
+        """Keeps path[b] (increasing indices into the tree of the last tree_attention, which nothing else followed) of every sequence: its
+        rows move to the end of the sequence, which grows by len(path[b]).  The rest of the tree is dropped; pages taken for it stay with
+        the sequence."""
         A = max((len(p) for p in path), default=0)
         if len(path) != self.B or any(list(p) != sorted(set(int(x) for x in p)) or (len(p) and p[0] < 0) for p in path):
             raise ValueError("path must hold, for each sequence, increasing non-negative tree indices")
-        pr = self.pool.page_rows
         for b, p in enumerate(path):
-            if len(p) and (self.lengths[b] + p[-1] >= self.max_pages * pr or self.table_host[b, (self.lengths[b] + p[-1]) // pr] < 0):
-                raise ValueError(f"path of sequence {b} names a token that was not drafted")
+            if len(p) and p[-1] >= self.drafted:
+                raise ValueError(f"path of sequence {b} names a token that was not drafted (the last tree has {self.drafted})")
         if A:
             flat = torch.full((self.B, A), -1, dtype=torch.int32)
             for b, p in enumerate(path):
@@ -126,6 +130,7 @@ class PagedFastForwardAttn:
             self.engine.tree_accept_per_sample(flat.to(self.table.device), self.table, self.rows)
             self.rows += torch.tensor([len(p) for p in path], dtype=torch.int32).to(self.rows.device)
         self.lengths = [n + len(p) for n, p in zip(self.lengths, path)]
+        self.drafted = 0
 
     @property
     def pages_in_use(self) -> int:
@@ -135,3 +140,4 @@ class PagedFastForwardAttn:
         self.pool.release(self.table_host[self.table_host >= 0].tolist())
         self.table_host.fill_(-1)
         self.table.fill_(-1)
+        self.drafted = 0
