@@ -308,6 +308,8 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
     // the smallest logit of a beam that can reach the bound, a little lower than it is so that rounding cannot lose one
     auto lowest = [&](int i) -> float {
         const double base = lse[i], s = (double)beam_score[i], need = bound - s + base;
+        if (s == CUDART_INF) return -CUDART_INF_F;       // every token of such a beam is as good as can be
+        if (bound == CUDART_INF) return CUDART_INF_F;    // and next to enough of them nothing else is
         return __double2float_rd(need - 1e-6 * (1.0 + fabs(bound) + fabs(s) + fabs(base)));
     };
     auto score_of = [&](int i, float x) -> double { return (double)beam_score[i] + ((double)x - lse[i]); };

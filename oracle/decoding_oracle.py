@@ -137,7 +137,7 @@ def beam_select(logits, scores, num, finished=None, pad_token=0):
             x = logits[b, i].double().cpu()
             if torch.isnan(x).any() or (x == math.inf).any() or not (s0 > -math.inf):
                 continue
-            s = s0 + (x - torch.logsumexp(x, 0))
+            s = torch.where(x > -math.inf, s0 + (x - torch.logsumexp(x, 0)), -math.inf)   # (+inf + -inf is no score either)
             cand += [(float(s[t]), i, t) for t in torch.argsort(s, descending=True, stable=True)[:num].tolist()]
         cand = sorted((c for c in cand if c[0] > -math.inf), key=lambda c: (-c[0], c[1], c[2]))
         rows.append((cand + [(-math.inf, 0, pad_token)] * num)[:num])

@@ -253,3 +253,19 @@ def test_short_vocabularies_and_few_live_beams(dt, B, beams, V, live, num):
         if live > 1:
             finished[:, 1] = True
         check(x, scores, num, finished, V - 1)
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+def test_select_infinitely_good_beams(dt):
+    """A score of +inf is above -inf: its beam's tokens are all equally good, the lowest first."""
+    logits, scores = candidates(dt, 4, 3, 700, seed=8)
+    scores[0, 1], scores[1, 0], scores[1, 2], scores[2, :], scores[3, 2] = INF, INF, INF, INF, INF
+    logits[0, 1, 1] = -INF                    # no candidate
+    finished = torch.zeros(4, 3, dtype=torch.bool, device="cuda")
+    finished[3, 2] = True
+    from fastforwardattention_b200 import beam_select
+
+    want, parents, tokens = D64.beam_select(logits, scores, 9, finished, 5)
+    got = beam_select(logits, scores, 9, finished=finished, pad_token=5)
+    assert torch.equal(got[1].cpu(), parents) and torch.equal(got[2].cpu(), tokens)
+    assert torch.equal(got[0].cpu() == INF, want == INF) and (want[0] == INF).all()
