@@ -26,12 +26,17 @@ namespace {
 //            the leader ranks the list and writes the result.
 // A CTA that notes more than its part of the list holds (a vocabulary of ties) finds its own num best by radix selection, 8 bits a
 // pass, over the 64-bit score and then the index: more than those cannot be in the result.
-// The sums of exponentials are fp32 per lane (a few dozen terms) and double across lanes and warps; scores are compared as
-// doubles, so that two beams' candidates a rounding of fp32 apart still come in the right order.
+// Exponentials are fp32; a lane adds 32 or 64 of them in fp32 and these sums, like those of lanes and warps, as doubles.  A log-sum is then off by
+// 3e-6 at most: 2^-22 for an exponential, (2^-24 + 1.5 2^-24) |x - reference| for its argument, whose mean under the softmax is at most about 11,
+// 11 2^-24 for the fp32 sums, 2^-22 for joining lanes and segments.  Scores are compared as doubles: tokens of one beam come in the exact order,
+// two beams' candidates whose scores lie closer than their log-sums' errors may come in either.
 constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelShare = 128;   // candidates that the leader's list holds of each CTA
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRaise = 8.f;    // a lane's sum is rescaled when a logit is this far above its reference: what it held is then a small part of
+                                 // the sum, and the errors of many rescalings (an ascending vocabulary) cannot add up
+constexpr int kFlush = 8;        // vectors that a lane adds in fp32
 
 struct SelRecord {       // one segment
     float m;             // largest logit, -inf: none
@@ -56,12 +61,6 @@ __device__ __forceinline__ void st_peer_v4(uint32_t addr, uint4 v)
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void st_peer_u32(uint32_t addr, unsigned v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ unsigned ld_peer_u32(uint32_t addr)
-{
-    unsigned v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
 
 // floats in the order of their values (no NaN), and back
 __device__ __forceinline__ uint32_t ordered32(float x)
@@ -204,24 +203,38 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
     const float s0 = works ? P.scores[(size_t)b * beams + beam] : -CUDART_INF_F;
     const bool alive = works && s0 > -CUDART_INF_F;   // a beam without a score has no candidates
 
-    float m = -CUDART_INF_F, l = 0.f;
+    float m = -CUDART_INF_F, ref = -CUDART_INF_F, l = 0.f;   // the lane's largest logit, what its terms are relative to, their newest ones' sum
+    double total = 0.0;                                       // and the others'
+    int adds = 0;
     if (alive && !done) {
         visit(row, vocab, seg * 32 + lane, segs * 32, [&](const float (&x)[EPV], int) {
             float top = x[0];
 #pragma unroll
             for (int e = 1; e < EPV; ++e) top = fmaxf(top, x[e]);
-            if (top > m) l *= fast_exp2((m - top) * kLog2e), m = top;
-            if (m == -CUDART_INF_F) {   // nothing yet, unless NaN hides among the -inf
+            m = fmaxf(m, top);
+            if (top > ref + kRaise) {
+                const float f = fast_exp2((ref - top) * kLog2e);
+                l *= f, total *= (double)f, ref = top;
+            }
+            if (ref == -CUDART_INF_F) {   // nothing yet, unless NaN hides among the -inf
 #pragma unroll
                 for (int e = 0; e < EPV; ++e) l += x[e] != x[e] ? CUDART_NAN_F : 0.f;
                 return;
             }
+            float t[EPV];
 #pragma unroll
-            for (int e = 0; e < EPV; ++e) l += fast_exp2((x[e] - m) * kLog2e);
+            for (int e = 0; e < EPV; ++e) t[e] = fast_exp2((x[e] - ref) * kLog2e);
+#pragma unroll
+            for (int n = EPV / 2; n >= 1; n /= 2)
+#pragma unroll
+                for (int e = 0; e < n; ++e) t[e] += t[e + n];
+            l += t[0];
+            if (++adds == kFlush) total += (double)l, l = 0.f, adds = 0;
         });
     } else if (alive && done && seg == 0) {
-        m = 0.f, l = lane == 0 ? 1.f : 0.f;   // a finished beam offers one candidate: its score as it is
+        m = ref = 0.f, l = lane == 0 ? 1.f : 0.f;   // a finished beam offers one candidate: its score as it is
     }
+    total += (double)l;
     SelRecord rec;
     {
         float t = m;
@@ -232,8 +245,8 @@ __global__ void __launch_bounds__(kSelThreads) ffa_beam_select_kernel(const FfaB
         rec.m = fmaxf(fmaxf(rec.quarter[0], rec.quarter[1]), fmaxf(rec.quarter[2], rec.quarter[3]));
         if (done) rec.quarter[1] = rec.quarter[2] = rec.quarter[3] = -CUDART_INF_F;
         rec.pad = 0.f;
-        // a lane without a finite logit adds its l (0, or NaN)
-        double sum = m == -CUDART_INF_F ? (double)l : (double)l * (double)expf(m - rec.m);
+        // a lane without a finite logit adds its total (0, or NaN)
+        double sum = ref == -CUDART_INF_F ? total : total * (double)expf(ref - rec.m);
 #pragma unroll
         for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         rec.l = sum;

@@ -269,3 +269,51 @@ def test_select_infinitely_good_beams(dt):
     got = beam_select(logits, scores, 9, finished=finished, pad_token=5)
     assert torch.equal(got[1].cpu(), parents) and torch.equal(got[2].cpu(), tokens)
     assert torch.equal(got[0].cpu() == INF, want == INF) and (want[0] == INF).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("B,N", [(1, 2), (149, 16)])
+def test_select_sums_of_long_vocabularies(dt, B, N):
+    """Equal terms whose fp32 sum would lose a part of the same sign at every addition: the scores are exact to one rounding and to what
+    the kernel states for the log-sum (here, with arguments of 0.3: 2^-22 + 0.3 x 2.5 x 2^-24 + 11 x 2^-24 + 2^-22 = 1.2e-6), and two beams that lie
+    further apart come in the right order."""
+    from fastforwardattention_b200 import beam_select
+
+    V = 50400
+    logits = torch.full((B, N, V), -0.3001, device="cuda").to(dt)
+    logits[:, :, :256] = 0.0                  # every lane starts with the largest logit
+    logits[:, 1, 256:] = torch.tensor(-0.3301, device="cuda").to(dt)
+    exact = torch.logsumexp(logits[0].double(), -1)
+    # the first beam's best tokens are 4e-6 better than the second's
+    scores = torch.full((B, N), -50.0, device="cuda")
+    scores[:, 0], scores[:, 1] = 0.0, (exact[1] - exact[0] - 4e-6).float()
+    s = scores[0].double()[:, None] + (0.0 - exact[:, None])
+    gap = float(s[0] - s[1])
+    assert 3.7e-6 < gap < 4.3e-6
+    best, parents, tokens = beam_select(logits, scores, 8)
+    assert (parents == 0).all() and (tokens == torch.arange(8, device="cuda")).all()
+    assert ((best.double() - s[0]).abs() <= D64.U * s[0].abs() + 1.2e-6).all()
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("kind", ["random", "ascending", "steep"])
+def test_select_log_sums_are_as_exact_as_stated(dt, kind):
+    """The kernel states 3e-6 for a log-sum, whatever the batch (the cluster of a sample shrinks with it) and the order of the logits."""
+    from fastforwardattention_b200 import beam_select
+
+    g = torch.Generator("cuda").manual_seed(9)
+    for B, N, V in [(1, 3, 50272), (40, 8, 50400), (149, 16, 50400)]:
+        if kind == "random":
+            logits = torch.randn(B, N, V, generator=g, device="cuda") * torch.linspace(0.5, 6, N, device="cuda")[:, None]
+        else:
+            ramp = torch.linspace(-1, 0, V, device="cuda") * (2.0 if kind == "ascending" else 300.0)
+            logits = ramp * torch.linspace(0.3, 1, N, device="cuda")[:, None] + torch.zeros(B, 1, 1, device="cuda")
+        logits = logits.to(dt)
+        scores = torch.randn(B, N, generator=g, device="cuda")
+        best, parents, tokens = beam_select(logits, scores, 8)
+        for b in (0, B - 1):
+            x = logits[b].double()
+            s = scores[b].double()[:, None] + (x - torch.logsumexp(x, -1, keepdim=True))
+            want = s[parents[b].long(), tokens[b].long()]
+            assert ((best[b].double() - want).abs() <= D64.U * want.abs() + 3e-6).all(), (kind, B)
+            assert (want >= s.flatten().topk(8).values - 6e-6).all()
