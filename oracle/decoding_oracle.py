@@ -48,9 +48,10 @@ def tree_attention(q, k, v, k_cache, v_cache, tree, scale, rows, first=None):
                 rel = 2 * dp + (n - lo + T + 8) * U
                 err = rel * a
                 if q.dtype != torch.float32:
-                    err = err + half_step(q.dtype) * a            # weights rounded to the tensors' type
-                    if q.dtype == torch.float16:                   # weights below fp16's normal range: half its smallest step each
-                        err = err + 2.0 ** -25 * torch.stack([vals[see[t]].abs().sum(0) for t in range(T)])
+                    # weights as sums of two numbers of the type; exponentials to 2.7e-6, in the weights and in their sum
+                    err = err + (half_step(q.dtype) ** 2 + 6e-6) * a
+                    if q.dtype == torch.float16:                   # parts of a weight below half of fp16's smallest step, at 2^7 times the weight
+                        err = err + 2.0 ** -32 * torch.stack([vals[see[t]].abs().sum(0) for t in range(T)])
                 bound[b, h * G + g] = err + half_step(q.dtype) * (o.abs() + err) + 1e-30
     return out, bound
 
