@@ -3,8 +3,8 @@
 // A CTA owns a tile of up to 128 query rows of one (batch, head) -- all drafted tokens of all query heads that share the
 // cache head -- and a run of key tiles of 64 rows.  Per tile
 //     S = Q K^T  [128 x 64]   fp32 in TMEM; Q and K are K-major operands in 128-byte-swizzled shared memory
-//     P = exp2(c S - m)       one thread per query row: TMEM -> registers -> P in two 16-bit parts back into S's columns
-//     O += P V   [128 x Dh]   A = P's parts from TMEM, B = V as it lies in the cache (MN-major)
+//     P = exp2(c S - m)       one thread per query row: TMEM -> registers -> 16-bit P back into S's columns
+//     O += P V   [128 x Dh]   A = P from TMEM, B = V as it lies in the cache (MN-major)
 // so a cache row is read from HBM once for all query rows.  The matrix units idle most of the time even with every product
 // padded to 128 rows (64 KB of K and V take 2.8 us of an SM's share of HBM, the products 0.5 us): what bounds a long cache is HBM.
 //
@@ -15,13 +15,14 @@
 // tree, and the chain of waits and instructions per tile, not a throughput, is what a softmax warp spends its time on.
 // The running maximum is raised lazily: weights are taken relative to a reference that follows the true maximum only when that
 // is more than 8 (in powers of two) ahead, so O is rarely rescaled and weights stay below 256, exact in either type's range.
-// A weight goes into the product as the sum of two numbers of the tensors' type, what it rounds to and what that leaves over, at the cost
-// of a second product per 16 keys: with one alone the result is 1.4 times as far from the exact one as its own rounding puts it (2.9e-4 against
-// 2.1e-4 in the 2-norm for fp16, 2.3e-3 against 1.7e-3 for bf16; the one-token step keeps fp32 weights), with both no further.  The second
-// product costs 6 % with up to 32 query rows (fp16, 320 pairs x 1237 x 64: 40.2 -> 42.7 us), 14 % and 20 % for 65 to 128 (128 pairs x 1920 x 256:
-// 65.6 -> 74.5; 16 pairs x 32705 x 128, two tiles of 66: 98 -> 118), 14 % with 33 to 64 (bf16, 1024 pairs x 8128 x 128: 745 -> 850; with the
-// parts in copies of the query rows of their own instead of a second product 12 % more than that, each thread then has twice the
-// exponentials.)  The sum is taken of the weights in fp32.
+// The sum is taken of the weights in fp32; what meets V is 16-bit.  With up to 32 query rows (a one-token step and most trees) a weight goes into the
+// product as the sum of two numbers of the type, what it rounds to and the rest, and the result is as close to the exact one as its own
+// rounding allows, like the one-token step's, whose weights are fp32: 2.1e-4 in the 2-norm for fp16, 1.7e-3 for bf16.  That costs a second
+// product per 16 keys, 6 % there (fp16, 320 pairs x 1237 x 64, 27 rows: 40.2 -> 42.7 us), where the chain of a tile's waits bounds.  With more rows the
+// products and, in a long loop, their power bound: 65.6 -> 77 us (128 pairs x 1920 x 256, 100 rows), 98 -> 120 (16 pairs x 32705 x 128, two tiles of 66)
+// and 745 -> 850 to 950 (bf16, 1024 pairs x 8128 x 128, 64 rows).  There a weight is rounded once, and the result is 1.4 times as far off: 2.9e-4 and
+// 2.3e-3.  (The rests in copies of the query rows of their own instead of a second product, 64 rows: 864 us where a second product takes 770 and
+// neither 700; each thread then has twice the exponentials.)
 #pragma once
 #include <cuda.h>
 
@@ -37,6 +38,7 @@ constexpr int kUmmaMaxStages = 12;
 constexpr int kQBoxRows = 32;      // Q arrives in boxes of 32 rows
 // copies of the query rows in a tile of the product
 constexpr int umma_rep(int tile_rows) { return tile_rows <= 32 ? 4 : tile_rows <= 64 ? 2 : 1; }
+constexpr bool umma_rests(int rep) { return rep == 4; }   // whether the weights' rests meet V too, see above
 constexpr float kLazyRescale = 8.f;
 constexpr int kFmaPairs = 3;       // of 8 pairs of exponentials, those that the FMA units take
 // fp16 weights are held 2^7 times as large (2^15 at most, the type ends at 65504): parts of a weight vanish below 2^-32 of the largest one
@@ -293,6 +295,8 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
     constexpr int BOX = 64 * 128;   // bytes of a tile's box: 64 rows of 128 bytes
     constexpr uint32_t S_COL = DP;  // TMEM columns: O at 0, the two S / P buffers behind it
     constexpr int QUADS = 4 / REP, COLS = kUmmaKeys / REP;   // warps per copy of the query rows; keys of a tile that a copy weighs
+    constexpr bool RESTS = umma_rests(REP);
+    constexpr int WORDS = RESTS ? 16 : 8;   // columns of P for 16 keys
     const FfaTreeParams& P = U.p;
     // No static shared memory: the dynamic part then starts on the 1024-byte boundary that swizzled operands need, without
     // slack (two CTAs with 112 KB of operands leave 1.5 KB of an SM)
@@ -399,9 +403,9 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
             const uint32_t p = tmem + S_COL + kUmmaKeys * (j & 1);
             if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kUmmaKeys / 16; ++k) {   // 16 keys: 8 + 8 columns of packed P, two atoms of V
-                    umma_ts(tmem, p + 16 * k, v + (2048 / 16) * k, O_DESC, j > 0 || k > 0);
-                    umma_ts(tmem, p + 16 * k + 8, v + (2048 / 16) * k, O_DESC, true);
+                for (int k = 0; k < kUmmaKeys / 16; ++k) {   // 16 keys: 8 columns of packed P (and 8 of the weights' rests), two atoms of V
+                    umma_ts(tmem, p + WORDS * k, v + (2048 / 16) * k, O_DESC, j > 0 || k > 0);
+                    if (RESTS) umma_ts(tmem, p + WORDS * k + 8, v + (2048 / 16) * k, O_DESC, true);
                 }
                 umma_commit(empty + 8 * stage);
                 umma_commit(pv_done + 8 * (j & 1));
@@ -540,7 +544,8 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
                 const float minus = m == -CUDART_INF_F ? 0.f : -m;
                 const float2 cc = make_float2(c, c), mm = make_float2(minus + weight_shift<T>(), minus + weight_shift<T>());
                 float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
-                uint32_t p[COLS];   // per 16 keys 8 words of the weights' first parts, then 8 of their second parts
+                constexpr int OWN = COLS / 16 * WORDS;
+                uint32_t p[OWN];   // per 16 keys 8 words of weights and then, if there are any, 8 of their rests
                 auto weigh = [&](auto fma_tag) {
 #pragma unroll
                     for (int i = 0; i < COLS / 2; ++i) {
@@ -548,9 +553,12 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
                         const float2 x = decltype(fma_tag)::value && i % 8 < kFmaPairs ? exp2_fma(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
                         if (i & 1) lb = __fadd2_rn(lb, x);
                         else la = __fadd2_rn(la, x);
-                        const uint32_t most = pack2<T>(x.x, x.y);
-                        const float2 rest = __ffma2_rn(unpack2<T>(most), make_float2(-1.f, -1.f), x);
-                        p[i / 8 * 16 + i % 8] = most, p[i / 8 * 16 + i % 8 + 8] = pack2<T>(rest.x, rest.y);
+                        const uint32_t w = pack2<T>(x.x, x.y);
+                        p[i / 8 * WORDS + i % 8] = w;
+                        if constexpr (RESTS) {
+                            const float2 rest = __ffma2_rn(unpack2<T>(w), make_float2(-1.f, -1.f), x);
+                            p[i / 8 * WORDS + i % 8 + 8] = pack2<T>(rest.x, rest.y);
+                        }
                     }
                 };
                 // where a score may be -inf its weight has to be 0, so that a row which sees nothing adds up to 0
@@ -559,19 +567,14 @@ __global__ void __launch_bounds__(kUmmaThreads, umma_ctas_per_sm(DH)) ffa_tree_u
                 l += (la.x + la.y) + (lb.x + lb.y);
                 if constexpr (REP == 1) {
                     tmem_st32<0>(s_addr, p);
-                    tmem_st32<32>(s_addr + 32, p);
                 } else {   // the other copies' keys get weight 0 in this one
-                    uint32_t none[COLS];
+                    static_assert(OWN == 16, "a share of the keys is 16 columns of P");
+                    uint32_t none[OWN];
 #pragma unroll
-                    for (int i = 0; i < COLS; ++i) none[i] = 0;
+                    for (int i = 0; i < OWN; ++i) none[i] = 0;
 #pragma unroll
-                    for (int i = 1; i < REP; ++i) {
-                        const uint32_t at = s_addr + ((rep + i) % REP) * COLS;
-                        if constexpr (REP == 2) tmem_st32<0>(at, none);
-                        else tmem_st16<0>(at, none);
-                    }
-                    if constexpr (REP == 2) tmem_st32<0>(s_addr + rep * 32, p);
-                    else tmem_st16<0>(s_addr + rep * 16, p);
+                    for (int i = 1; i < REP; ++i) tmem_st16<0>(s_addr + ((rep + i) % REP) * OWN, none);
+                    tmem_st16<0>(s_addr + rep * OWN, p);
                 }
                 if (masked) {
                     // What V holds outside the valid rows, and infinities and NaN of drafted tokens, must not meet a weight of 0:

@@ -190,8 +190,8 @@ int ffa_attention_paged(ffa_plan_t* plan, const void* q, const void* k, const vo
  * A query row that sees nothing is 0.  A token that a row does not see has no influence on it, whatever its values.
  * An infinity in a visible row of V, cached or drafted, is one in the result (fp32: as long as the row's weight is a number of fp32 above
  * 0), infinities of both signs or NaN are NaN.
- * Statistics and sums are fp32; fp16 and bf16 weights meet V with twice the type's bits (as sums of two numbers of the type), and the result
- * is rounded once.
+ * Statistics and sums are fp32 and the result is rounded once; fp16 and bf16 weights meet V as sums of two numbers of the type with up to 32 query
+ * rows (groups * tokens), and rounded to the type with more.
  * groups * tokens <= 1024.  page_table: NULL, or the paged caches of ffa_attention_paged with pools of pool_pages pages; every page
  * that holds rows 0..row+tokens-1 of a sequence has to be in its table (a sequence with an entry outside [0, pool_pages) there is
  * refused: FFA_STATUS_BAD_INDEX, output zero, nothing appended).

@@ -48,9 +48,10 @@ def tree_attention(q, k, v, k_cache, v_cache, tree, scale, rows, first=None):
                 rel = 2 * dp + (n - lo + T + 8) * U
                 err = rel * a
                 if q.dtype != torch.float32:
-                    # weights as sums of two numbers of the type; exponentials to 2.7e-6, in the weights and in their sum
-                    err = err + (half_step(q.dtype) ** 2 + 6e-6) * a
-                    if q.dtype == torch.float16:                   # parts of a weight below half of fp16's smallest step, at 2^7 times the weight
+                    # weights rounded to the tensors' type, with up to 32 query rows as sums of two numbers of it; exponentials to 2.7e-6, in the weights and
+                    # in their sum
+                    err = err + (half_step(q.dtype) ** (2 if G * T <= 32 else 1) + 6e-6) * a
+                    if q.dtype == torch.float16:                   # what is below half of fp16's smallest step, of 2^7 times a weight
                         err = err + 2.0 ** -32 * torch.stack([vals[see[t]].abs().sum(0) for t in range(T)])
                 bound[b, h * G + g] = err + half_step(q.dtype) * (o.abs() + err) + 1e-30
     return out, bound

@@ -469,26 +469,28 @@ def test_an_infinity_in_a_cached_row_is_one_in_the_result(dt, D, T, n):
     D64.assert_within(out, want, bound)
 
 
-def close_bound(q, k, v, k_cache, v_cache, tree, scale, rows):
-    """The exact result, and how far a kernel may be from it whose weights have more bits than the tensors' type: the fp32 bound, and of
-    a = sum p |v| the square of a half step (a weight is the sum of two numbers of the type) and 6e-6 (the exponentials' 2.7e-6 in the weights and
-    in their sum); in fp16 parts of a weight below 2^-25 vanish, which is 2^-32 of the largest one; then one rounding of the result."""
+def close_bound(q, k, v, k_cache, v_cache, tree, scale, rows, top=1.0):
+    """The exact result, and how far a kernel may be from it: the fp32 bound, and of a = sum p |v| a half step for weights rounded to the type, or its
+    square for weights that are sums of two numbers of it (up to 32 query rows), and 6e-6 (the exponentials' 2.7e-6 in the weights and in their
+    sum); in fp16, whose weights are held at 2^7 times their size, what is below 2^-25 of that
+    vanishes, 2^-32 of the largest weight (`top`: of all); then one rounding of the result."""
     wide = [x.float() for x in (q, k, v, k_cache, v_cache)]
     out, err = D64.tree_attention(*wide, tree, scale, rows)
     a, _ = D64.tree_attention(*wide[:2], wide[2].abs(), wide[3], wide[4].abs(), tree, scale, rows)
     h = D64.half_step(q.dtype)
-    err = err + (h * h + 6e-6) * a
+    few = q.shape[1] // k.shape[1] * q.shape[2] <= 32
+    err = err + ((h * h if few else h) + 6e-6) * a
     if q.dtype == torch.float16:
         n = max(rows)
-        err = err + 2.0 ** -32 * (wide[4][:, :, :n].abs().sum(2).amax() + wide[2].abs().sum(2).amax())
+        err = err + 2.0 ** -32 * top * (wide[4][:, :, :n].abs().sum(2).amax() + wide[2].abs().sum(2).amax())
     return out, err + h * (out.abs() + err)
 
 
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("D", [64, 80, 128, 256])
-@pytest.mark.parametrize("G,T,n", [(1, 1, 700), (1, 8, 63), (1, 27, 1000), (2, 25, 400), (1, 100, 300), (4, 33, 5000)])
+@pytest.mark.parametrize("G,T,n", [(1, 1, 700), (1, 8, 63), (1, 27, 1000), (2, 16, 400), (4, 8, 5000), (1, 33, 300), (1, 100, 300)])
 def test_weights_keep_more_bits_than_the_tensors(dt, D, G, T, n):
-    """The only rounding to the tensors' type is the result's, as in the one-token step."""
+    """With up to 32 query rows the only rounding to the tensors' type is the result's, as in the one-token step."""
     ffa, kc, vc, q, k, v, tree = setup(dt, 2, 2, G, D, n, T, seed=T + n)
     want, bound = close_bound(q, k, v, kc, vc, tree, D ** -0.5, [n, n])
     D64.assert_within(ffa.tree_attention(q, k, v, tree, D ** -0.5, n), want, bound)
@@ -497,21 +499,18 @@ def test_weights_keep_more_bits_than_the_tensors(dt, D, G, T, n):
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("T", [1, 40, 70])
 @pytest.mark.parametrize("units", [6.5, 40.5, 300.5, 1200.5])
-def test_many_light_keys_beside_a_heavy_one(dt, T, units):
-    """An attention sink: a key with a small value, and 16384 others that have `units` steps of fp16 below its normal range (2^-24) of its
-    weight each.  As many pairs as let every one be walked by one CTA, whose largest weight is then the sink's."""
-    H, D, n = 320, 64, 16384
+def test_many_light_keys_beside_heavy_ones(dt, T, units):
+    """Attention sinks: every 256th key takes a weight of 1 and has no value, each of the others has `units` of fp16's smallest steps (2^-24), and
+    the result is theirs alone: what is lost of their weights shows whole."""
+    H, D, n = 2, 64, 16384
     ffa, kc, vc, q, k, v, tree = setup(dt, 1, H, 1, D, n, T, seed=T)
-    scale = math.log(2.0 ** 24 / units) / D   # q . k of the sink: D
-    q.fill_(1.0), kc.zero_()
-    kc[:, :, 5] = 1.0
-    k *= 0.1
+    scale = math.log(2.0 ** 24 / units) / D   # q . k of a sink: D
+    q.fill_(1.0), kc.zero_(), k.zero_()
+    kc[:, :, ::256] = 1.0
     vc += 1.0
-    vc[:, :, 5] *= 0.01
-    last = lambda x: x[:, -1:]
-    want, bound = close_bound(*map(last, (q, k, v, kc, vc)), tree, scale, [n])
-    out = ffa.tree_attention(q, k, v, tree, scale, n)
-    D64.assert_within(last(out), want, bound)
+    vc[:, :, ::256] = 0.0
+    want, bound = close_bound(q, k, v, kc, vc, tree, scale, [n], top=256 / n)
+    D64.assert_within(ffa.tree_attention(q, k, v, tree, scale, n), want, bound)
 
 
 def test_paths_that_repeat_an_index_at_the_end_of_a_paged_sequence():
