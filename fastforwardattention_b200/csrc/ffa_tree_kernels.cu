@@ -103,7 +103,9 @@ void ffa_k_tree_shape(int dtype, int head_dim, int rows, FfaTreeShape* s)
         const bool few = simt_few(head_dim, rows);
         s->tile_rows = few ? (rows <= 8 ? 8 : 16) : 16 * simt_rt(rows), s->tile_keys = kTreeKeys;
         const int fit = kSmemPerSm / (simt_smem(head_dim, rows) + 1024);
-        const int most = few ? (rows <= 8 ? 3 : 2) : 4;   // by registers
+        // by registers: 168 and 255 a thread of 128; of 256 threads Dh 64 has 75 a thread with two rows to a thread and 134 with four (the
+        // other head sizes: shared memory is the tighter limit, or the same)
+        const int most = few ? (rows <= 8 ? 3 : 2) : head_dim == 64 ? (simt_rt(rows) == 4 ? 1 : 3) : 4;
         s->ctas_per_sm = fit > most ? most : fit;
         // S and O of a tile: 4 * rows * keys * Dh flops at about 55 % of an SM's 128 FMAs a cycle (30 % with a warp a scheduler), and two
         // memory latencies

@@ -102,3 +102,18 @@ def test_reorder_refusals(plan, kw, code):
     a = dict(plan=p, kc=P16, vc=P16, parents=P16, beams=4, first=0, rows=50, stream=None)
     a.update(kw)
     assert L.ffa_cache_reorder(*a.values()) == code, L.ffa_last_error()
+
+
+@pytest.mark.parametrize("T,resident", [(20, 3), (32, 3), (40, 1), (64, 1), (100, 1)])
+def test_fp32_trees_are_split_for_the_ctas_that_their_registers_allow(T, resident):
+    """Head_dim 64, 17 query rows and more: 75 registers for each of 256 threads with two rows to a thread, 134 with four.  A split over more CTAs than
+    are resident would run in waves."""
+    L = capi.lib()
+    p, n = C.c_void_p(), C.c_size_t()
+    capi.check(L.ffa_plan_create_offline(capi.F32, 1, 32, 64, 5000, 0, SMS, SMEM_CTA, SMEM_SM, C.byref(p)))
+    capi.check(L.ffa_tree_scratch_bytes(p, 1, T, 4000, C.byref(n)))
+    tile = 32 if T <= 32 else 64
+    tiles, rows = -(-T // tile), min(T, tile)
+    splits = n.value // (32 * tiles * rows * (64 + 4) * 4)
+    assert splits > 1 and 32 * tiles * splits <= SMS * resident
+    L.ffa_plan_destroy(p)
