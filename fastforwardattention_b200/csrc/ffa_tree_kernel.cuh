@@ -4,7 +4,7 @@
 //                                   (visible where tree[t(r), j]); r = (query head of the group, drafted token)
 //   O[r]    = sum_j exp(S[r, j] - m_r) v_j / sum_j exp(S[r, j] - m_r);  a row that sees nothing is 0
 //
-// The drafted tokens are read from the call's k and v and appended to the cache by one CTA of the pair, so no CTA ever
+// The drafted tokens are read from the call's k and v; the pair's CTAs append them to the cache (fp16, bf16: one of them does), so no CTA ever
 // waits for another one's append.
 #pragma once
 #include "ffa_device_common.cuh"
@@ -346,10 +346,10 @@ __global__ void __launch_bounds__(kTreeThreads) ffa_tree_simt_kernel(const FfaTr
 //       then added over the slices so that a lane is left with one row.  (With whole columns and 2 rows x 2 keys to a lane, 4 products
 //       to 4 reads, the kernel waits for shared memory.)
 //   O   lane = columns: all rows x DH / 32 columns, the weights broadcast from shared memory (Dh 64: half a warp each takes every other key)
-// Each warp has its own running maximum and sum; the warps meet once, at the end.  Bound by HBM while there are many pairs and at most
-// 8 rows, then by latency and shared memory.  This kernel and the one above, each at its number of splits: 256 pairs x 2000 tokens x
-// 128, 6 drafted 100 / 178 us (floor 81), 16 drafted 175 / 350; 16 pairs x 8000 x 80, 5 drafted 31 / 41; 32 pairs x 995 x 64, 5 drafted and
-// accepted 14.9 / 15.0, 12 drafted 17.3 / 17.0.
+// Each warp has its own running maximum and sum; the warps meet once, at the end.  With head_dim 128, many pairs and at most 8 rows HBM bounds,
+// otherwise latency and shared memory (256 pairs x 2000 x 64, 6 drafted: 83 us at a floor of 40).  This kernel and the one above, each at its number of
+// splits: 256 pairs x 2000 tokens x 128, 6 drafted 100 / 178 us (floor 81), 16 drafted 175 / 350; 16 pairs x 8000 x 80, 5 drafted 31 / 41;
+// 32 pairs x 995 x 64, 5 drafted and accepted 14.9 / 15.0, 12 drafted 17.3 / 17.0.
 constexpr int kFewWarps = 4, kFewKeys = 16;   // keys a warp and tile
 constexpr int few_kv_floats(int dh) { return 2 * kFewKeys * dh; }   // K and V of a warp
 constexpr int few_stages(int dh) { return dh <= 64 ? 2 : 1; }   // as many as leave room for three CTAs to an SM (by registers two, with 16 rows)

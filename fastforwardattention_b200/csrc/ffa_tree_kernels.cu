@@ -1,5 +1,6 @@
 // Launch glue of the tree attention: fp16 and bf16 on the tensor cores (ffa_tree_umma_kernel.cuh), fp32 on the CUDA cores
-// (ffa_tree_kernel.cuh; the tensor cores have no product of fp32's precision), and the acceptance of a path.
+// (ffa_tree_kernel.cuh; the tensor cores round fp32 operands to tf32, and products of operands split into several such parts were not tried), and
+// the acceptance of a path.
 #include "ffa_tree_kernel.cuh"
 #include "ffa_tree_umma_kernel.cuh"
 

@@ -5,8 +5,9 @@
 //     S = Q K^T  [128 x 64]   fp32 in TMEM; Q and K are K-major operands in 128-byte-swizzled shared memory
 //     P = exp2(c S - m)       one thread per query row: TMEM -> registers -> 16-bit P back into S's columns
 //     O += P V   [128 x Dh]   A = P from TMEM, B = V as it lies in the cache (MN-major)
-// so a cache row is read from HBM once for all query rows.  The matrix units idle most of the time even with every product
-// padded to 128 rows (64 KB of K and V take 2.8 us of an SM's share of HBM, the products 0.5 us): what bounds a long cache is HBM.
+// so a cache row is read from HBM once for all query rows.  A tile of 64 keys x 128 is 32 KB, 1400 cycles of an SM's share of HBM, and about 650
+// of products, although half of each and more is padding or copies (256 pairs x 4096, 64 query rows: tensor pipe active 40 % of the time, DRAM at 72 %
+// of its peak with starts and ends): what bounds a long cache is HBM.
 //
 // Warps: 0 issues the TMA loads, 1 allocates TMEM and issues the products, 2..5 do the softmax (a warp can only reach the 32 TMEM
 // lanes of its rank modulo 4).  S has two buffers, so that S of the next tile is computed while the softmax of this one runs.

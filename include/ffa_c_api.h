@@ -215,7 +215,7 @@ int ffa_tree_accept(ffa_plan_t* plan, void* k_cache, void* v_cache, const int* p
  *   weights[b, h, r] += p[r] for the cached rows, weights[b, h, row] = p[row] and positions[b, h, row] = seen[b] for the new one
  * (row = t, or seq_lengths[b] as in ffa_attention with right padding; t is then their bound).  weights [batch, heads, max_len] fp32,
  * positions [batch, heads, max_len] int32 or NULL, seen [batch] int32 or NULL (the row index).  The workspace must be sized with
- * with_scores = 1.
+ * with_scores = 1, or the scores bound beside it (ffa_workspace_bind_scores).
  * ffa_evict then keeps `keep` rows of every pair that has more: sample b uses rows 0..rows[b]-1, rows[b] <= max_rows <= 2^19.  Rows
  * with a position below `first`, or among the `recent` newest positions (above the pair's largest position - recent), stay; of the others the heaviest
  * stay, ties going to the lower row (NaN counts as the lightest; should more than `keep` rows be protected, the lowest of them stay).
