@@ -6,7 +6,7 @@
 //     P = exp2(c S - m)       one thread per query row: TMEM -> registers -> 16-bit P back into S's columns
 //     O += P V   [128 x Dh]   A = P from TMEM, B = V as it lies in the cache (MN-major)
 // so a cache row is read from HBM once for all query rows.  A tile of 64 keys x 128 is 32 KB, 1400 cycles of an SM's share of HBM, and about 650
-// of products, although half of each and more is padding or copies (256 pairs x 4096, 64 query rows: tensor pipe active 40 % of the time, DRAM at 72 %
+// of products, although half of each and more is padding or copies (256 pairs x 4096, 64 query rows: tensor pipe active 40 % of the time, DRAM at 71 %
 // of its peak with starts and ends): what bounds a long cache is HBM.
 //
 // Warps: 0 issues the TMA loads, 1 allocates TMEM and issues the products, 2..5 do the softmax (a warp can only reach the 32 TMEM
